@@ -9,7 +9,7 @@ import ctypes
 from ctypes import c_char_p, c_float, c_int32, c_int64, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 
-ABI_VERSION = 3
+ABI_VERSION = 4
 FLAG_FORCE_GENERIC = 1
 FLAG_PREFER_STREAM = 2
 FLAG_ACCUMULATE_DV = 4
@@ -63,6 +63,29 @@ SIGNATURES = {
         c_void_p, c_int32,
         c_void_p, c_void_p,
         c_uint32, c_void_p]),
+    "attnres_b200_norm_forward": (c_int32, [
+        c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_float,
+        c_void_p, c_void_p, c_void_p]),
+    "attnres_b200_norm_workspace_rows": (c_int32, [c_int64, c_int32, c_int32]),
+    "attnres_b200_norm_backward": (c_int32, [
+        c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int32, c_int32,
+        c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p]),
+    "attnres_b200_embedding_forward": (c_int32, [
+        c_void_p, c_int32, c_int64, c_int64, c_int32, c_int32, c_void_p, c_int64, c_int32,
+        c_void_p, c_int64, c_int32, c_float, c_void_p, c_int32, c_void_p]),
+    "attnres_b200_embedding_workspace_bytes": (c_int64, [c_int64, c_int32]),
+    "attnres_b200_embedding_backward": (c_int32, [
+        c_void_p, c_int32, c_int64, c_int64, c_int32, c_int32, c_int64, c_void_p, c_int64, c_int32,
+        c_float, c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_int64, c_void_p]),
+    "attnres_b200_loss_workspace_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32]),
+    "attnres_b200_loss_forward": (c_int32, [
+        c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_int32, c_int32,
+        c_int32, c_int64, c_float, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "attnres_b200_loss_backward": (c_int32, [
+        c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_int32, c_int32,
+        c_int32, c_int64, c_float, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
 }
 
 _library = None
@@ -210,3 +233,49 @@ def selftest_wait_limit(scratch_ptr, limit_ns, stream) -> None:
 
 def kernel_family(S, D, R, aligned, backward_pass) -> str:
     return load().attnres_b200_kernel_family(S, D, R, int(aligned), int(backward_pass)).decode()
+
+
+def _sized(value: int, what: str) -> int:
+    """A size query's answer; a negative one is a status."""
+    if value < 0:
+        check(-value, what)
+    return value
+
+
+def norm_forward(*arguments) -> None:
+    check(load().attnres_b200_norm_forward(*arguments), "attnres_b200_norm_forward")
+
+
+def norm_workspace_rows(N, D, device_index) -> int:
+    return _sized(load().attnres_b200_norm_workspace_rows(N, D, device_index),
+                  "attnres_b200_norm_workspace_rows")
+
+
+def norm_backward(*arguments) -> None:
+    check(load().attnres_b200_norm_backward(*arguments), "attnres_b200_norm_backward")
+
+
+def embedding_forward(*arguments) -> None:
+    check(load().attnres_b200_embedding_forward(*arguments), "attnres_b200_embedding_forward")
+
+
+def embedding_workspace_bytes(N, D) -> int:
+    return _sized(load().attnres_b200_embedding_workspace_bytes(N, D),
+                  "attnres_b200_embedding_workspace_bytes")
+
+
+def embedding_backward(*arguments) -> None:
+    check(load().attnres_b200_embedding_backward(*arguments), "attnres_b200_embedding_backward")
+
+
+def loss_workspace_bytes(N, V, D, backward_pass) -> int:
+    return _sized(load().attnres_b200_loss_workspace_bytes(N, V, D, int(backward_pass)),
+                  "attnres_b200_loss_workspace_bytes")
+
+
+def loss_forward(*arguments) -> None:
+    check(load().attnres_b200_loss_forward(*arguments), "attnres_b200_loss_forward")
+
+
+def loss_backward(*arguments) -> None:
+    check(load().attnres_b200_loss_backward(*arguments), "attnres_b200_loss_backward")

@@ -1,26 +1,28 @@
 """Build the sm_100a shared library in-tree: ``python fast-attnres_b200/build.py``.
 
-One ``nvcc`` invocation compiles ``csrc/attnres_b200.cu`` (which includes the
-kernel headers) into ``attnres/_lib/libattnres_b200.so``.  nvcc cross-compiles
+One ``nvcc`` invocation compiles the translation units of ``csrc`` (the read, LayerNorm,
+embedding and the vocabulary loss; each includes its kernel headers), side by side, into ``attnres/_lib/libattnres_b200.so``.  nvcc cross-compiles
 for sm_100a, so no GPU is needed to build.
 """
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 ROOT = Path(__file__).resolve().parent
-SOURCES = [ROOT / "csrc" / "attnres_b200.cu"]
+SOURCES = [ROOT / "csrc" / name for name in ("attnres_b200.cu", "norm.cu", "embedding.cu", "loss.cu")]
 HEADERS = sorted((ROOT / "csrc").glob("*.cuh")) + [ROOT.parent / "include" / "attnres_b200.h"]
 OUTPUT = ROOT / "attnres" / "_lib" / "libattnres_b200.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
     "--expt-relaxed-constexpr",
 ]
 
@@ -39,20 +41,47 @@ def up_to_date() -> bool:
     return all(path.stat().st_mtime <= built for path in [*SOURCES, *HEADERS, Path(__file__)])
 
 
+def _includes(path: Path, seen: set[Path]) -> set[Path]:
+    """`path` and every project header it includes, directly or not."""
+    path = path.resolve()
+    if path not in seen and path.exists():
+        seen.add(path)
+        for name in re.findall(r'#include "([^"]+)"', path.read_text()):
+            _includes(path.parent / name, seen)
+    return seen
+
+
+def _compile(source: Path, force: bool) -> tuple[Path, str]:
+    """Compile one translation unit; returns its object file and what the compiler said."""
+    target = OUTPUT.parent / (source.stem + ".o")
+    newest = max(path.stat().st_mtime for path in [*_includes(source, set()), Path(__file__)])
+    if not force and target.exists() and newest <= target.stat().st_mtime:
+        return target, ""
+    # ptxas always reports registers and spills (shown only when asked for): the flag also
+    # fixes the order in which it lays the kernels out, so every build of the same sources
+    # gives the same binary whether or not the report is printed.
+    return target, _run([_nvcc(), *NVCC_FLAGS, "-Xptxas", "-v", "-c", str(source), "-o", str(target)])
+
+
+def _run(command: list[str]) -> str:
+    result = subprocess.run(command, capture_output=True, text=True)
+    if result.returncode != 0:
+        sys.stderr.write(result.stdout + result.stderr)
+        raise RuntimeError(f"nvcc failed with exit code {result.returncode}")
+    return result.stdout + result.stderr
+
+
 def build(*, force: bool = False, verbose: bool = False) -> Path:
     """Compile the library if any source is newer than it; return its path."""
     if not force and up_to_date():
         return OUTPUT
     OUTPUT.parent.mkdir(parents=True, exist_ok=True)
-    # ptxas always reports registers and spills (shown only when asked for): the flag also
-    # fixes the order in which it lays the kernels out, so every build of the same sources
-    # gives the same binary whether or not the report is printed.
-    command = [_nvcc(), *NVCC_FLAGS, "-Xptxas", "-v", *map(str, SOURCES), "-o", str(OUTPUT)]
-    result = subprocess.run(command, capture_output=True, text=True)
-    if verbose or result.returncode != 0:
-        sys.stderr.write(result.stdout + result.stderr)
-    if result.returncode != 0:
-        raise RuntimeError(f"nvcc failed with exit code {result.returncode}")
+    with ThreadPoolExecutor(len(SOURCES)) as pool:
+        compiled = list(pool.map(lambda source: _compile(source, force), SOURCES))
+    if verbose:
+        sys.stderr.write("".join(text for _, text in compiled))
+    _run([_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-shared",
+          *(str(target) for target, _ in compiled), "-o", str(OUTPUT)])
     return OUTPUT
 
 

@@ -7,6 +7,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "host_common.cuh"
 #include "generic_kernels.cuh"
 #include "fwd_ring_kernel.cuh"
 #include "bwd_stash_kernel.cuh"
@@ -14,31 +15,10 @@
 #include "bwd_stream_kernel.cuh"
 
 namespace attnres_b200 {
+
+int loss_error_flag(int* flag, int clear);  // loss.cu
+
 namespace {
-
-int sm_count(int device, int* out) {
-  // Queried per call: the attribute lookup is a cached driver read and keeps
-  // the library free of mutable global state.
-  int sms = 0;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
-      sms < 1) {
-    cudaGetLastError();
-    return ATTNRES_B200_ERR_CUDA;
-  }
-  *out = sms;
-  return ATTNRES_B200_OK;
-}
-
-int current_device(int* device) {
-  if (cudaGetDevice(device) != cudaSuccess) {
-    cudaGetLastError();
-    return ATTNRES_B200_ERR_CUDA;
-  }
-  return ATTNRES_B200_OK;
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
 
 int check_shape(int32_t S, int64_t N, int32_t D, int32_t R) {
   if (S < 1 || S > kMaxSources) return ATTNRES_B200_ERR_BAD_SOURCE_COUNT;
@@ -239,6 +219,8 @@ extern "C" const char* attnres_b200_status_string(int status) {
     case ATTNRES_B200_ERR_STATIC_SCRATCH:
       return "shape needs more dquery scratch than the built-in array holds; pass a workspace to "
              "attnres_b200_backward";
+    case ATTNRES_B200_ERR_BAD_TYPE: return "an element type the operator does not take";
+    case ATTNRES_B200_ERR_BAD_VOCABULARY: return "vocabulary outside 1..2^25";
     default: return "unknown status";
   }
 }
@@ -277,6 +259,9 @@ extern "C" int attnres_b200_error_flag(int32_t* flag, int32_t clear) {
       return ATTNRES_B200_ERR_CUDA;
     }
   }
+  int loss = 0;  // the products of the vocabulary loss raise a flag of their own
+  if (int st = loss_error_flag(&loss, clear)) return st;
+  *flag |= loss;
   return ATTNRES_B200_OK;
 }
 

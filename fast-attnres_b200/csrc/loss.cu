@@ -1,0 +1,332 @@
+// C ABI of the vocabulary loss (declared in include/attnres_b200.h).
+#include <cmath>
+#include <mutex>
+
+#include "loss_kernels.cuh"
+
+namespace attnres_b200 {
+
+int loss_error_flag(int* flag, int clear) {
+  int value = 0;
+  if (cudaMemcpyFromSymbol(&value, g_error_flag, sizeof(int)) != cudaSuccess) {
+    cudaGetLastError();
+    return ATTNRES_B200_ERR_CUDA;
+  }
+  *flag = value;
+  if (clear && value != 0) {
+    const int zero = 0;
+    if (cudaMemcpyToSymbol(g_error_flag, &zero, sizeof(int)) != cudaSuccess) {
+      cudaGetLastError();
+      return ATTNRES_B200_ERR_CUDA;
+    }
+  }
+  return ATTNRES_B200_OK;
+}
+
+namespace {
+
+constexpr int64_t kMaxLossRows = 1 << 30;
+constexpr int32_t kMaxLossVocabulary = 1 << 25;
+// Rows whose (max, sum) pairs are held at a time (65 536 x 250 pairs at 32 000 ids: 131 MB).
+constexpr int64_t kStatsRows = 65536;
+// Bytes of P held at a time.  A larger piece means fewer passes over the FP32 sums of dH; at
+// 16 384 rows two pieces cover 32 000 ids.
+constexpr int64_t kPieceBytes = 512ll << 20;
+constexpr int64_t kPieceMinimum = 4096;
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+  static std::once_flag once;
+  static EncodeTiled function = nullptr;
+  std::call_once(once, [] {
+    void* found = nullptr;
+    cudaDriverEntryPointQueryResult result;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &found, 12000, cudaEnableDefault,
+                                         &result) == cudaSuccess &&
+        result == cudaDriverEntryPointSuccess)
+      function = reinterpret_cast<EncodeTiled>(found);
+    else
+      cudaGetLastError();
+  });
+  return function;
+}
+
+// A 16-bit row-major matrix read (or written) in boxes of 64 columns.
+int make_map(CUtensorMap* map, const void* base, int32_t type, int64_t rows, int64_t columns,
+             int64_t row_stride, int box_rows) {
+  EncodeTiled encode = encode_tiled();
+  if (encode == nullptr) return ATTNRES_B200_ERR_CUDA;
+  const cuuint64_t sizes[2] = {(cuuint64_t)columns, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)row_stride * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, steps[2] = {1, 1};
+  const CUtensorMapDataType element = type == ATTNRES_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return encode(map, element, 2, const_cast<void*>(base), sizes, strides, box, steps,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+                 CUDA_SUCCESS
+             ? ATTNRES_B200_OK
+             : ATTNRES_B200_ERR_CUDA;
+}
+
+int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+int check_loss(int64_t N, int32_t V, int32_t D, int32_t type, float scale) {
+  if (D < 1 || D > kMaxWidth) return ATTNRES_B200_ERR_BAD_WIDTH;
+  if (N < 1 || N > kMaxLossRows) return ATTNRES_B200_ERR_BAD_ROWS;
+  if (V < 1 || V > kMaxLossVocabulary) return ATTNRES_B200_ERR_BAD_VOCABULARY;
+  if (type != ATTNRES_B200_BF16 && type != ATTNRES_B200_FP16) return ATTNRES_B200_ERR_BAD_TYPE;
+  if (!std::isfinite(scale)) return ATTNRES_B200_ERR_BAD_SCALAR;
+  return ATTNRES_B200_OK;
+}
+
+int32_t padded_width(int32_t D) { return (D + 7) / 8 * 8; }
+
+bool needs_padding(const void* weight, int64_t row_stride, int32_t V, int32_t D) {
+  return D % 8 != 0 || !aligned16(weight) || (V > 1 && (row_stride % 8 != 0 || row_stride < D));
+}
+
+struct LossPlan {
+  int64_t padded_weight;  // bytes of a padded copy of the weight
+  int64_t stats_rows, partials;
+  int64_t piece, pieces;  // ids of a piece
+  int64_t probs, running, weights;
+};
+
+LossPlan plan_loss(int64_t N, int32_t V, int32_t D) {
+  LossPlan plan;
+  plan.padded_weight = align256((int64_t)V * padded_width(D) * 2);
+  plan.stats_rows = N < kStatsRows ? N : kStatsRows;
+  const int64_t tiles_n = (V + kTileN - 1) / kTileN;
+  plan.partials = align256(plan.stats_rows * 2 * tiles_n * (int64_t)sizeof(float2));
+  int64_t most = kPieceBytes / (2 * N) / kTileN * kTileN;
+  if (most < kPieceMinimum) most = kPieceMinimum;
+  plan.pieces = (V + most - 1) / most;
+  plan.piece = ((V + plan.pieces - 1) / plan.pieces + kTileN - 1) / kTileN * kTileN;
+  plan.pieces = (V + plan.piece - 1) / plan.piece;
+  const int64_t columns = plan.piece < V ? plan.piece : padded_width(V);
+  plan.probs = align256(N * columns * 2);
+  plan.running = plan.pieces > 1 ? align256(N * D * (int64_t)sizeof(float)) : 0;
+  plan.weights = align256((N + 1) * (int64_t)sizeof(float));
+  return plan;
+}
+
+template <int PASS, typename T>
+int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& p_map,
+                   const ProductParams& p, int64_t tiles, int sms, cudaStream_t stream) {
+  static SmemGrant grant;
+  if (int st = prepare_kernel(loss_product_kernel<PASS, T>, kProductSmem, grant)) return st;
+  const int grid = (int)(tiles < sms ? tiles : sms);
+  loss_product_kernel<PASS, T><<<grid, kProductThreads, kProductSmem, stream>>>(a, b, p_map, p);
+  return launched();
+}
+
+template <int PASS>
+int launch_product_type(int32_t type, const CUtensorMap& a, const CUtensorMap& b,
+                        const CUtensorMap& p_map, const ProductParams& p, int64_t tiles, int sms,
+                        cudaStream_t stream) {
+  return type == ATTNRES_B200_BF16
+             ? launch_product<PASS, __nv_bfloat16>(a, b, p_map, p, tiles, sms, stream)
+             : launch_product<PASS, __half>(a, b, p_map, p, tiles, sms, stream);
+}
+
+int64_t tiles_of(int64_t rows, int64_t columns) {
+  return ((rows + kTileM - 1) / kTileM) * ((columns + kTileN - 1) / kTileN);
+}
+
+// The weight as the TMA can read it: in place, or copied into rows of a multiple of eight.
+int lay_out_weight(const void** weight, int64_t* row_stride, int32_t V, int32_t D, void* copy,
+                   int sms, cudaStream_t stream) {
+  if (!needs_padding(*weight, *row_stride, V, D)) return ATTNRES_B200_OK;
+  loss_pad_kernel<<<sms * 8, 256, 0, stream>>>(static_cast<unsigned short*>(copy),
+                                               static_cast<const unsigned short*>(*weight),
+                                               *row_stride, V, D, padded_width(D));
+  *weight = copy;
+  *row_stride = padded_width(D);
+  return launched();
+}
+
+}  // namespace
+}  // namespace attnres_b200
+
+using namespace attnres_b200;
+
+extern "C" int64_t attnres_b200_loss_workspace_bytes(int64_t N, int32_t V, int32_t D,
+                                                     int32_t backward) {
+  if (int st = check_loss(N, V, D, ATTNRES_B200_BF16, 1.f)) return -st;
+  const LossPlan plan = plan_loss(N, V, D);
+  if (!backward) return plan.padded_weight + plan.partials + align256(N * (int64_t)sizeof(float));
+  return plan.padded_weight + plan.probs + plan.running + plan.weights;
+}
+
+extern "C" int attnres_b200_loss_forward(
+    const void* hidden, int64_t hidden_row_stride, const void* weight, int64_t weight_row_stride,
+    const void* targets, int32_t targets_64, int64_t N, int32_t V, int32_t D, int32_t type,
+    int64_t ignored, float scale, int32_t reduction, void* kept, int32_t* kept_index,
+    int32_t* kept_target, int32_t* count, float* lse2, float* losses, float* loss, void* workspace,
+    int64_t workspace_bytes, void* stream) {
+  if (int st = check_loss(N, V, D, type, scale)) return st;
+  if (reduction < ATTNRES_B200_LOSS_NONE || reduction > ATTNRES_B200_LOSS_MEAN)
+    return ATTNRES_B200_ERR_BAD_FLAGS;
+  if (!hidden || !weight || !targets || !kept || !kept_index || !kept_target || !count || !lse2 ||
+      !losses || !workspace || (reduction != ATTNRES_B200_LOSS_NONE && !loss))
+    return ATTNRES_B200_ERR_NULL_POINTER;
+  if (!aligned2(hidden) || !aligned2(weight) || !aligned16(kept) || !aligned16(workspace) ||
+      (reinterpret_cast<uintptr_t>(targets) & (targets_64 ? 7u : 3u)) != 0)
+    return ATTNRES_B200_ERR_MISALIGNED;
+  if (workspace_bytes < attnres_b200_loss_workspace_bytes(N, V, D, 0))
+    return ATTNRES_B200_ERR_WORKSPACE;
+  int device = 0, sms = 0;
+  if (int st = current_device(&device)) return st;
+  if (int st = sm_count(device, &sms)) return st;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  const LossPlan plan = plan_loss(N, V, D);
+  const int32_t Dp = padded_width(D);
+  char* space = static_cast<char*>(workspace);
+  float2* partials = reinterpret_cast<float2*>(space + plan.padded_weight);
+  float* target_logit = reinterpret_cast<float*>(space + plan.padded_weight + plan.partials);
+
+  GatherParams g{};
+  g.hidden = hidden;
+  g.hidden_row_stride = hidden_row_stride;
+  g.targets = targets;
+  g.targets_64 = targets_64;
+  g.N = N;
+  g.D = D;
+  g.Dp = Dp;
+  g.V = V;
+  g.ignored = ignored;
+  // Every CTA counts the kept rows before its own, so their number is bounded (512).
+  g.block_rows = (int32_t)(32 * ((N + 32 * 512 - 1) / (32 * 512)));
+  g.kept = static_cast<unsigned short*>(kept);
+  g.kept_index = kept_index;
+  g.kept_target = kept_target;
+  g.count = count;
+  g.target_logit = target_logit;
+  g.losses = losses;
+  const int gather_grid = (int)((N + g.block_rows - 1) / g.block_rows);
+  if (D % 8 == 0 && aligned16(hidden) && (N == 1 || hidden_row_stride % 8 == 0))
+    loss_gather_kernel<true><<<gather_grid, kGatherThreads, 0, cs>>>(g);
+  else
+    loss_gather_kernel<false><<<gather_grid, kGatherThreads, 0, cs>>>(g);
+  if (int st = launched()) return st;
+  if (int st = lay_out_weight(&weight, &weight_row_stride, V, D, space, sms, cs)) return st;
+
+  CUtensorMap map_h, map_w;
+  if (int st = make_map(&map_h, kept, type, N, D, Dp, 64)) return st;
+  if (int st = make_map(&map_w, weight, type, V, D, V > 1 ? weight_row_stride : Dp, 64)) return st;
+  ProductParams p{};
+  p.count = count;
+  p.N = (int32_t)N;
+  p.V = V;
+  p.D = D;
+  p.v0 = 0;
+  p.vn = V;
+  p.scale = scale;
+  p.kept_target = kept_target;
+  p.partials = partials;
+  p.target_logit = target_logit;
+  const int pairs = 2 * ((V + kTileN - 1) / kTileN);
+  for (int64_t row = 0; row < N; row += plan.stats_rows) {
+    p.first_row = (int32_t)row;
+    p.row_limit = (int32_t)(N - row < plan.stats_rows ? N - row : plan.stats_rows);
+    if (int st = launch_product_type<kStats>(type, map_h, map_w, map_w, p, tiles_of(p.row_limit, V),
+                                             sms, cs))
+      return st;
+    loss_join_kernel<<<(p.row_limit + 7) / 8, 256, 0, cs>>>(partials, pairs, count, p.first_row,
+                                                            p.row_limit, target_logit, kept_index,
+                                                            lse2, losses);
+    if (int st = launched()) return st;
+  }
+  if (reduction == ATTNRES_B200_LOSS_NONE) return ATTNRES_B200_OK;
+  loss_reduce_kernel<<<1, 1024, 0, cs>>>(losses, N, count, reduction == ATTNRES_B200_LOSS_MEAN, loss);
+  return launched();
+}
+
+extern "C" int attnres_b200_loss_backward(
+    const float* upstream, int64_t upstream_stride, const void* weight, int64_t weight_row_stride,
+    const void* targets, int32_t targets_64, int64_t N, int32_t V, int32_t D, int32_t type,
+    int64_t ignored, float scale, int32_t reduction, const void* kept, const int32_t* kept_index,
+    const int32_t* kept_target, const int32_t* count, const float* lse2, void* dhidden,
+    void* dweight, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int st = check_loss(N, V, D, type, scale)) return st;
+  if (reduction < ATTNRES_B200_LOSS_NONE || reduction > ATTNRES_B200_LOSS_MEAN)
+    return ATTNRES_B200_ERR_BAD_FLAGS;
+  if (!dhidden && !dweight) return ATTNRES_B200_ERR_NOTHING_TO_DO;
+  if (!upstream || !weight || !targets || !kept || !kept_index || !kept_target || !count || !lse2 ||
+      !workspace)
+    return ATTNRES_B200_ERR_NULL_POINTER;
+  if (!aligned2(weight) || !aligned16(kept) || !aligned16(workspace) || !aligned2(dhidden) ||
+      !aligned2(dweight) || (reinterpret_cast<uintptr_t>(targets) & (targets_64 ? 7u : 3u)) != 0)
+    return ATTNRES_B200_ERR_MISALIGNED;
+  if (workspace_bytes < attnres_b200_loss_workspace_bytes(N, V, D, 1))
+    return ATTNRES_B200_ERR_WORKSPACE;
+  int device = 0, sms = 0;
+  if (int st = current_device(&device)) return st;
+  if (int st = sm_count(device, &sms)) return st;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  const LossPlan plan = plan_loss(N, V, D);
+  const int32_t Dp = padded_width(D);
+  char* space = static_cast<char*>(workspace);
+  void* probs = space + plan.padded_weight;
+  float* running = reinterpret_cast<float*>(space + plan.padded_weight + plan.probs);
+  float* gradient_scale =
+      reinterpret_cast<float*>(space + plan.padded_weight + plan.probs + plan.running);
+  float* weight_of = gradient_scale + 1;
+
+  if (int st = lay_out_weight(&weight, &weight_row_stride, V, D, space, sms, cs)) return st;
+  const int64_t zero_ctas = (N + 31) / 32;
+  loss_weights_kernel<<<1 + (int)(zero_ctas < 2 * sms ? zero_ctas : 2 * sms), 1024, 0, cs>>>(
+      upstream, upstream_stride, reduction == ATTNRES_B200_LOSS_NONE,
+      reduction == ATTNRES_B200_LOSS_MEAN, count, kept_index,
+      type == ATTNRES_B200_FP16 ? kHalfLift : 1.f, weight_of, gradient_scale, targets, targets_64,
+      ignored, N, static_cast<unsigned short*>(dhidden), D);
+  if (int st = launched()) return st;
+
+  CUtensorMap map_h, map_w;
+  if (int st = make_map(&map_h, kept, type, N, D, Dp, 64)) return st;
+  if (int st = make_map(&map_w, weight, type, V, D, V > 1 ? weight_row_stride : Dp, 64)) return st;
+  ProductParams p{};
+  p.count = count;
+  p.N = (int32_t)N;
+  p.V = V;
+  p.D = D;
+  p.scale = scale;
+  p.kept_index = kept_index;
+  p.kept_target = kept_target;
+  p.lse2 = lse2;
+  p.weight_of = weight_of;
+  p.gradient_scale = gradient_scale;
+  p.running = running;
+  for (int64_t v0 = 0; v0 < V; v0 += plan.piece) {
+    p.v0 = (int32_t)v0;
+    p.vn = (int32_t)(V - v0 < plan.piece ? V - v0 : plan.piece);
+    p.first_piece = v0 == 0;
+    p.last_piece = v0 + p.vn == V;
+    CUtensorMap map_p, map_p_store;
+    const int64_t stride = padded_width(p.vn);
+    if (int st = make_map(&map_p, probs, type, N, p.vn, stride, 64)) return st;
+    if (int st = make_map(&map_p_store, probs, type, N, p.vn, stride, 32)) return st;
+    if (int st = launch_product_type<kProbs>(type, map_h, map_w, map_p_store, p, tiles_of(N, p.vn),
+                                             sms, cs))
+      return st;
+    if (dhidden != nullptr) {
+      p.out = dhidden;
+      p.vector_out = D % 8 == 0 && aligned16(dhidden);
+      if (int st = launch_product_type<kHidden>(type, map_p, map_w, map_p, p, tiles_of(N, D), sms, cs))
+        return st;
+    }
+    if (dweight != nullptr) {
+      p.out = dweight;
+      p.vector_out = D % 8 == 0 && aligned16(dweight);
+      if (int st = launch_product_type<kWeight>(type, map_p, map_h, map_p, p, tiles_of(p.vn, D), sms,
+                                                cs))
+        return st;
+    }
+  }
+  return ATTNRES_B200_OK;
+}

@@ -1,0 +1,601 @@
+// Softmax cross entropy of z = scale * H W^T against target ids, without keeping z.
+//
+//   lse_n = log sum_v exp(z_nv)          loss_n = lse_n - z_n,target
+//   P_nv  = c_n (exp(z_nv - lse_n) - [v = target_n])     c_n: what the loss of row n weighs
+//   dH    = scale P W                    dW = scale P^T H
+//
+// Every product runs on the tensor cores with FP32 accumulators:
+//   kStats   tiles of z in tensor memory, reduced at once to a (max, sum) pair per row and half
+//            tile; a second kernel joins the pairs.  z never leaves the SM.
+//   kProbs   the same tiles again, turned into P (16-bit, the inputs' type) for one piece of the
+//            vocabulary;
+//   kHidden  dH from the piece, kWeight the piece's rows of dW.
+// Forming z twice costs a quarter of the training pass's products and saves [N, V] of memory.
+//
+// Rows whose target is the ignored id take no part: the kept rows are first gathered into
+// consecutive ones (their number stays on the device), so padding costs no products and whatever
+// an ignored row holds, infinities included, reaches no result.
+#pragma once
+
+#include "tcgen05.cuh"
+#include "typed_access.cuh"
+
+namespace attnres_b200 {
+
+// ------------------------------------------------------------------------------ gathering rows
+
+struct GatherParams {
+  const void* hidden;       // 16-bit [N, D], feature stride 1
+  int64_t hidden_row_stride;
+  const void* targets;
+  int32_t targets_64;
+  int64_t N;
+  int32_t D, Dp;            // Dp: D rounded up to eight
+  int32_t V;
+  int64_t ignored;
+  int32_t block_rows;
+  unsigned short* kept;     // [N, Dp]: the kept rows, zeros up to the next multiple of 128 rows
+  int32_t* kept_index;      // [N]: their rows in the input
+  int32_t* kept_target;     // [N]: their targets, -1 when outside the vocabulary
+  int32_t* count;
+  float* target_logit;      // [N], to be filled in by the products
+  float* losses;            // [N]: zero for ignored rows
+};
+
+__device__ __forceinline__ int64_t load_target(const void* targets, int wide, int64_t n) {
+  return wide ? __ldg(static_cast<const long long*>(targets) + n)
+              : (int64_t)__ldg(static_cast<const int*>(targets) + n);
+}
+
+// One 16-bit row of D elements into a 16-byte aligned one of Dp, by one warp; NULL: zeros.
+template <bool VECTOR>
+__device__ __forceinline__ void copy_row(unsigned short* dst, const unsigned short* src, int D,
+                                         int Dp, int lane) {
+  if (VECTOR && src != nullptr) {
+#pragma unroll 4
+    for (int c = lane; c < Dp / 8; c += 32)
+      reinterpret_cast<uint4*>(dst)[c] = __ldg(reinterpret_cast<const uint4*>(src) + c);
+  } else {
+#pragma unroll 4
+    for (int i = lane; i < Dp; i += 32)
+      dst[i] = (src != nullptr && i < D) ? __ldg(src + i) : (unsigned short)0;
+  }
+}
+
+constexpr int kGatherThreads = 1024;
+
+template <bool VECTOR>
+__global__ void __launch_bounds__(kGatherThreads) loss_gather_kernel(const GatherParams p) {
+  __shared__ int warp_counts[kGatherThreads / 32];
+  __shared__ int places[kGatherThreads];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t first = (int64_t)blockIdx.x * p.block_rows;
+  const int64_t last = min(p.N, first + p.block_rows);
+  // Kept rows before this CTA's: every CTA counts them for itself.
+  int before = 0;
+#pragma unroll 4
+  for (int64_t n = tid; n < first; n += kGatherThreads)
+    before += load_target(p.targets, p.targets_64, n) != p.ignored;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (lane == 0) warp_counts[warp] = before;
+  __syncthreads();
+  int place = 0;
+  for (int w = 0; w < kGatherThreads / 32; ++w) place += warp_counts[w];
+  __syncthreads();
+  for (int64_t base = first; base < last; base += kGatherThreads) {
+    const int64_t n = base + tid;
+    const int64_t target = n < last ? load_target(p.targets, p.targets_64, n) : p.ignored;
+    const bool keep = n < last && target != p.ignored;
+    const uint32_t votes = __ballot_sync(0xffffffffu, keep);
+    if (lane == 0) warp_counts[warp] = __popc(votes);
+    __syncthreads();
+    int mine = place, total = 0;
+    for (int w = 0; w < kGatherThreads / 32; ++w) {
+      if (w < warp) mine += warp_counts[w];
+      total += warp_counts[w];
+    }
+    mine += __popc(votes & ((1u << lane) - 1u));
+    places[tid] = keep ? mine : -1;
+    if (keep) {
+      p.kept_index[mine] = (int32_t)n;
+      p.kept_target[mine] = (target >= 0 && target < p.V) ? (int32_t)target : -1;
+      p.target_logit[mine] = __int_as_float(0x7fc00000);  // stays when there is no such logit
+    } else if (n < last) {
+      p.losses[n] = 0.f;
+    }
+    __syncthreads();
+    const int rows = (int)min((int64_t)kGatherThreads, last - base);
+    for (int r = warp; r < rows; r += kGatherThreads / 32) {
+      if (places[r] >= 0)
+        copy_row<VECTOR>(p.kept + (int64_t)places[r] * p.Dp,
+                         static_cast<const unsigned short*>(p.hidden) +
+                             (base + r) * p.hidden_row_stride,
+                         p.D, p.Dp, lane);
+    }
+    place += total;
+    __syncthreads();
+  }
+  if (last == p.N) {  // the last CTA knows how many there are
+    if (tid == 0) *p.count = place;
+    const int64_t padded = min(p.N, ((int64_t)place + 127) / 128 * 128);
+    for (int64_t r = place + warp; r < padded; r += kGatherThreads / 32)
+      copy_row<VECTOR>(p.kept + r * p.Dp, nullptr, p.D, p.Dp, lane);
+  }
+}
+
+// A weight whose rows the TMA cannot take (width or alignment) is laid out with rows of Dp.
+__global__ void __launch_bounds__(256)
+loss_pad_kernel(unsigned short* dst, const unsigned short* src, int64_t row_stride, int64_t rows,
+                int D, int Dp) {
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8)
+    copy_row<false>(dst + r * Dp, src + r * row_stride, D, Dp, threadIdx.x & 31);
+}
+
+// ------------------------------------------------------------------------------ the products
+
+enum LossPass { kStats, kProbs, kHidden, kWeight };
+
+constexpr int kTileM = 128, kTileN = 256, kTileK = 64;
+constexpr int kBoxBytes = 64 * 64 * 2;
+constexpr int kStageBytes = (kTileM + kTileN) / 64 * kBoxBytes;  // 48 KB
+constexpr int kStages = 4;
+constexpr int kEpilogueWarps = 8;
+constexpr int kProductThreads = 64 + kEpilogueWarps * 32;
+constexpr int kStoreBytes = 32 * 64 * 2;  // a warp's 32 x 64 block of P
+constexpr uint32_t kProductSmem = kStages * kStageBytes + kEpilogueWarps * kStoreBytes + 1024;
+// FP16 keeps P times 2^15: probabilities of a large vocabulary would be subnormal.
+constexpr float kHalfLift = 32768.f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct ProductParams {
+  const int32_t* count;  // kept rows
+  int32_t N, V, D;
+  int32_t first_row;     // kStats: rows [first_row, first_row + row_limit)
+  int32_t row_limit;
+  int32_t v0, vn;        // the piece: ids [v0, v0 + vn)
+  float scale;
+  const int32_t* kept_index;
+  const int32_t* kept_target;
+  float2* partials;        // kStats: [row_limit][2 tiles_n] (max, sum) in powers of two
+  float* target_logit;     // kStats: scale * log2(e) * z of the target
+  const float* lse2;       // kProbs: log2 of the sum of exponentials
+  const float* weight_of;  // kProbs: c_n over gradient_scale[0]
+  const float* gradient_scale;  // kHidden, kWeight
+  void* out;               // kHidden: [N, D]; kWeight: [V, D]
+  float* running;          // kHidden: FP32 [N, D] sums over the pieces (more than one piece)
+  int32_t first_piece, last_piece;
+  int32_t vector_out;      // rows of `out` allow 16-byte stores
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  return pack_bf16x2(lo, hi);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  return pack_half2(lo, hi);
+}
+
+// Tiles in the order in which CTAs take them.  z: sixteen row tiles share each column tile while
+// it is in L2.  Gradients: the few column tiles of a row tile run side by side, so P is read once.
+template <int PASS>
+__device__ __forceinline__ void tile_at(int index, int tiles_m, int tiles_n, int* m, int* n) {
+  if constexpr (PASS == kStats || PASS == kProbs) {
+    constexpr int kGroup = 16;
+    const int group = index / (kGroup * tiles_n), rest = index - group * kGroup * tiles_n;
+    const int height = min(kGroup, tiles_m - group * kGroup);
+    *n = rest / height;
+    *m = group * kGroup + rest - *n * height;
+  } else {
+    *m = index / tiles_n;
+    *n = index - *m * tiles_n;
+  }
+}
+
+// Warp 0 loads, warp 1 multiplies, warps 2..9 take finished tiles out of tensor memory while the
+// next one is formed in its other half.
+template <int PASS, typename T>
+__global__ void __launch_bounds__(kProductThreads, 1)
+loss_product_kernel(const __grid_constant__ CUtensorMap map_a,
+                    const __grid_constant__ CUtensorMap map_b,
+                    const __grid_constant__ CUtensorMap map_p, const ProductParams p) {
+  constexpr bool kAmn = PASS == kWeight, kBmn = PASS == kHidden || PASS == kWeight;
+  constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
+  constexpr uint32_t kInstruction = mma_instruction(kBf16, kAmn, kBmn, kTileM, kTileN);
+  extern __shared__ unsigned char product_smem[];
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], done[2], taken[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t stages = (smem_addr(product_smem) + 1023u) & ~1023u;
+
+  const int kept = *p.count;
+  int tiles_m, tiles_n, k_steps;
+  if constexpr (PASS == kStats || PASS == kProbs) {
+    const int rows = PASS == kStats ? min(max(kept - p.first_row, 0), p.row_limit) : kept;
+    tiles_m = (rows + kTileM - 1) / kTileM;
+    tiles_n = (p.vn + kTileN - 1) / kTileN;
+    k_steps = (p.D + kTileK - 1) / kTileK;
+  } else if constexpr (PASS == kHidden) {
+    tiles_m = (kept + kTileM - 1) / kTileM;
+    tiles_n = (p.D + kTileN - 1) / kTileN;
+    k_steps = (p.vn + kTileK - 1) / kTileK;
+  } else {
+    tiles_m = (p.vn + kTileM - 1) / kTileM;
+    tiles_n = (p.D + kTileN - 1) / kTileN;
+    k_steps = (kept + kTileK - 1) / kTileK;
+  }
+  const int tiles = tiles_m * tiles_n;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&done[b], 1);
+      mbar_init(&taken[b], kEpilogueWarps);
+    }
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_tensor_map(&map_a);
+    prefetch_tensor_map(&map_b);
+  }
+  if (warp == 1) tmem_alloc_512(&tmem_slot);
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool alive = true;
+      for (int i = blockIdx.x; i < tiles && alive; i += gridDim.x) {
+        int m, n;
+        tile_at<PASS>(i, tiles_m, tiles_n, &m, &n);
+        // Where the operands' rows (K-major) or columns (MN-major) of this tile begin.
+        const int a0 = PASS == kStats ? p.first_row + m * kTileM : m * kTileM;
+        const int b0 = (PASS == kStats || PASS == kProbs) ? p.v0 + n * kTileN : n * kTileN;
+        const int bk = PASS == kHidden ? p.v0 : 0;
+        for (int k = 0; k < k_steps; ++k) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, &abort_flag)) {
+            alive = false;
+            break;
+          }
+          mbar_expect_tx(&full[stage], kStageBytes);
+          const uint32_t a = stages + stage * kStageBytes, b = a + kTileM / 64 * kBoxBytes;
+#pragma unroll
+          for (int j = 0; j < kTileM / 64; ++j) {
+            if constexpr (kAmn) tensor_load_2d(a + j * kBoxBytes, &map_a, a0 + j * 64, k * kTileK, &full[stage]);
+            else tensor_load_2d(a + j * kBoxBytes, &map_a, k * kTileK, a0 + j * 64, &full[stage]);
+          }
+#pragma unroll
+          for (int j = 0; j < kTileN / 64; ++j) {
+            if constexpr (kBmn) tensor_load_2d(b + j * kBoxBytes, &map_b, b0 + j * 64, bk + k * kTileK, &full[stage]);
+            else tensor_load_2d(b + j * kBoxBytes, &map_b, k * kTileK, b0 + j * 64, &full[stage]);
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0, buffer = 0;
+      uint32_t phase = 0, buffer_phase = 0;
+      bool alive = true;
+      for (int i = blockIdx.x; i < tiles && alive; i += gridDim.x) {
+        if (!mbar_wait(&taken[buffer], buffer_phase ^ 1u, &abort_flag)) break;
+        tcgen05_fence_after();
+        const uint32_t d = tmem + buffer * kTileN;
+        for (int k = 0; k < k_steps; ++k) {
+          if (!mbar_wait(&full[stage], phase, &abort_flag)) {
+            alive = false;
+            break;
+          }
+          tcgen05_fence_after();
+          const uint32_t a = stages + stage * kStageBytes, b = a + kTileM / 64 * kBoxBytes;
+          // 16 elements of K: 32 bytes along a K-major row, two 1 KB groups of MN-major rows.
+          const uint64_t da = operand_descriptor(a), db = operand_descriptor(b);
+#pragma unroll
+          for (int kk = 0; kk < kTileK / 16; ++kk)
+            tcgen05_mma_f16(d, da + kk * (kAmn ? 2048 >> 4 : 32 >> 4),
+                            db + kk * (kBmn ? 2048 >> 4 : 32 >> 4), kInstruction, k > 0 || kk > 0);
+          tcgen05_commit(&empty[stage]);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!alive) break;
+        tcgen05_commit(&done[buffer]);
+        buffer ^= 1;
+        if (buffer == 0) buffer_phase ^= 1u;
+      }
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t staging = stages + kStages * kStageBytes + (warp - 2) * kStoreBytes;
+    const float to_log2 = p.scale * kLog2e;
+    float out_scale = 0.f;
+    if constexpr (PASS == kHidden || PASS == kWeight)
+      out_scale = p.scale * *p.gradient_scale * (kBf16 ? 1.f : 1.f / kHalfLift);
+    int buffer = 0;
+    uint32_t buffer_phase = 0;
+    for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
+      int m, n;
+      tile_at<PASS>(i, tiles_m, tiles_n, &m, &n);
+      const int row = m * kTileM + quad * 32 + lane;  // of the tile's matrix
+      const int column = n * kTileN + half * (kTileN / 2);
+      // What the row needs is fetched while the products run.
+      int target = -1;
+      float lse2 = 0.f, weight_of = 0.f;
+      bool live = true;
+      if constexpr (PASS == kStats) {
+        live = p.first_row + row < kept && row < p.row_limit;
+        if (live) target = p.kept_target[p.first_row + row];
+      } else if constexpr (PASS == kProbs) {
+        live = row < kept;
+        if (live) {
+          target = p.kept_target[row];
+          target = target >= p.v0 ? target - p.v0 : -1;
+          lse2 = p.lse2[row];
+          weight_of = p.weight_of[row];
+        }
+      }
+      if (!mbar_wait(&done[buffer], buffer_phase, &abort_flag)) break;
+      tcgen05_fence_after();
+      const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + buffer * kTileN + half * (kTileN / 2);
+      if constexpr (PASS == kStats) {
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < kTileN / 2 && column + c < p.vn; c += 32) {
+          uint32_t r[32];
+          tmem_load_32(src + c, r);
+          float y[32], high = top;
+          const int valid = p.vn - column - c;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            y[e] = e < valid ? __uint_as_float(r[e]) * to_log2 : -INFINITY;
+            high = fmaxf(high, y[e]);
+          }
+          const int at = target - column - c;
+          if (at >= 0 && at < 32) {
+            float z = y[0];
+#pragma unroll
+            for (int e = 1; e < 32; ++e) z = at == e ? y[e] : z;
+            p.target_logit[p.first_row + row] = z;
+          }
+          // A row of nothing but -inf so far: subtract zero, its terms are exp2(-inf) = 0.
+          const float pivot = high == -INFINITY ? 0.f : high;
+          float part = 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) part += exp2_approx(y[e] - pivot);
+          sum = fmaf(sum, exp2_approx(top - pivot), part);
+          top = high;
+        }
+        if (live) p.partials[(int64_t)row * (2 * tiles_n) + 2 * n + half] = make_float2(top, sum);
+      } else if constexpr (PASS == kProbs) {
+        const bool rows_exist = m * kTileM + quad * 32 < p.N;
+#pragma unroll 1
+        for (int c = 0; c < kTileN / 2 && column + c < p.vn; c += 64) {
+          if (lane == 0) tensor_store_wait_read();
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t r[32];
+            tmem_load_32(src + c + h * 32, r);
+            const int at = target - column - c - h * 32;
+            float v[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float prob = exp2_approx(fmaf(__uint_as_float(r[e]), to_log2, -lse2));
+              v[e] = weight_of * (at == e ? prob - 1.f : prob);
+            }
+            if (!live) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = 0.f;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t w0 = pack2<T>(v[8 * q], v[8 * q + 1]);
+              const uint32_t w1 = pack2<T>(v[8 * q + 2], v[8 * q + 3]);
+              const uint32_t w2 = pack2<T>(v[8 * q + 4], v[8 * q + 5]);
+              const uint32_t w3 = pack2<T>(v[8 * q + 6], v[8 * q + 7]);
+              const uint32_t slot = staging + lane * 128 + (((h * 4 + q) ^ (lane & 7)) << 4);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot), "r"(w0), "r"(w1),
+                           "r"(w2), "r"(w3)
+                           : "memory");
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && rows_exist)
+            tensor_store_2d(&map_p, column + c, m * kTileM + quad * 32, staging);
+        }
+      } else {
+        const int rows = PASS == kHidden ? kept : p.vn;
+        int64_t out_row = 0;
+        if (row < rows) out_row = PASS == kHidden ? p.kept_index[row] : p.v0 + row;
+        T* out = static_cast<T*>(p.out) + out_row * p.D;
+        float* running = PASS == kHidden ? p.running + (int64_t)row * p.D : nullptr;
+#pragma unroll 1
+        for (int c = 0; c < kTileN / 2 && column + c < p.D; c += 32) {
+          uint32_t r[32];
+          tmem_load_32(src + c, r);
+          float v[32];
+          const int base = column + c, valid = min(32, p.D - base);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = k_steps > 0 ? __uint_as_float(r[e]) : 0.f;
+          if (row < rows) {
+            if (PASS == kHidden && !p.first_piece) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (e < valid) v[e] += running[base + e];
+            }
+            if (PASS == kHidden && !p.last_piece) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (e < valid) running[base + e] = v[e];
+            } else if (p.vector_out) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                if (8 * q < valid) {
+                  uint4 w;
+                  w.x = pack2<T>(v[8 * q] * out_scale, v[8 * q + 1] * out_scale);
+                  w.y = pack2<T>(v[8 * q + 2] * out_scale, v[8 * q + 3] * out_scale);
+                  w.z = pack2<T>(v[8 * q + 4] * out_scale, v[8 * q + 5] * out_scale);
+                  w.w = pack2<T>(v[8 * q + 6] * out_scale, v[8 * q + 7] * out_scale);
+                  *reinterpret_cast<uint4*>(out + base + 8 * q) = w;
+                }
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (e < valid) out[base + e] = from_float<T>(v[e] * out_scale);
+            }
+          }
+        }
+      }
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&taken[buffer]);
+      buffer ^= 1;
+      if (buffer == 0) buffer_phase ^= 1u;
+    }
+    if (PASS == kProbs && lane == 0) tensor_store_wait_read();
+  }
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  if (abort_flag != 0) {  // copies and products still in flight land before anything is given back
+    const uint64_t start = global_timer_ns();
+    while (global_timer_ns() - start < 200000ull) {
+    }
+    __syncthreads();
+  }
+  if (warp == 1) tmem_dealloc_512(tmem);
+}
+
+// ------------------------------------------------------------------------------ joining the loss
+
+// One warp per kept row: log2 of the row's sum of exponentials from its (max, sum) pairs.
+__global__ void __launch_bounds__(256)
+loss_join_kernel(const float2* __restrict__ partials, int pairs, const int32_t* count, int first_row,
+                 int row_limit, const float* __restrict__ target_logit,
+                 const int32_t* __restrict__ kept_index, float* __restrict__ lse2,
+                 float* __restrict__ losses) {
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= row_limit || first_row + row >= *count) return;
+  const float2* mine = partials + (int64_t)row * pairs;
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+  for (int i = lane; i < pairs; i += 32) {
+    const float2 v = mine[i];
+    const float high = fmaxf(top, v.x), pivot = high == -INFINITY ? 0.f : high;
+    sum = sum * exp2f(top - pivot) + v.y * exp2f(v.x - pivot);
+    top = high;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float other_top = __shfl_xor_sync(0xffffffffu, top, o);
+    const float other_sum = __shfl_xor_sync(0xffffffffu, sum, o);
+    const float high = fmaxf(top, other_top), pivot = high == -INFINITY ? 0.f : high;
+    sum = sum * exp2f(top - pivot) + other_sum * exp2f(other_top - pivot);
+    top = high;
+  }
+  if (lane == 0) {
+    const float at_target = target_logit[first_row + row];
+    // No logit at the target (an id outside the vocabulary): the loss and the gradients of the
+    // row are not numbers, so the mistake shows.
+    float joined = top + log2f(sum);
+    if (isnan(at_target)) joined = at_target;
+    lse2[first_row + row] = joined;
+    losses[kept_index[first_row + row]] = (joined - at_target) * kLn2;
+  }
+}
+
+// Sum or mean of the losses, in a fixed order and FP64, by one CTA.
+__global__ void __launch_bounds__(1024)
+loss_reduce_kernel(const float* __restrict__ losses, int64_t N, const int32_t* count, int mean,
+                   float* out) {
+  __shared__ double sums[32];
+  double sum = 0.0;
+#pragma unroll 4
+  for (int64_t n = threadIdx.x; n < N; n += 1024) sum += (double)losses[n];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double total = 0.0;
+    for (int w = 0; w < 32; ++w) total += sums[w];
+    *out = (float)(mean ? total / (double)*count : total);  // no kept row: not a number
+  }
+}
+
+// ------------------------------------------------------------------------------ before the gradients
+
+// What each kept row's loss weighs in the result, as a factor of at most one (times 2^15 for
+// FP16) and one common scale that the products apply in FP32: whatever the upstream gradient is,
+// P stays within its type.  CTA 0 does this; the others zero the gradient of ignored rows.
+__global__ void __launch_bounds__(1024)
+loss_weights_kernel(const float* upstream, int64_t upstream_stride, int per_row, int mean,
+                    const int32_t* count, const int32_t* __restrict__ kept_index, float lift,
+                    float* __restrict__ weight_of, float* gradient_scale, const void* targets,
+                    int targets_64, int64_t ignored, int64_t N, unsigned short* dhidden, int D) {
+  const int tid = threadIdx.x;
+  if (blockIdx.x > 0) {
+    if (dhidden == nullptr) return;
+    const int lane = tid & 31;
+    for (int64_t n = (int64_t)(blockIdx.x - 1) * 32 + (tid >> 5); n < N;
+         n += (int64_t)(gridDim.x - 1) * 32) {
+      if (load_target(targets, targets_64, n) == ignored)
+        for (int i = lane; i < D; i += 32) dhidden[n * D + i] = 0;
+    }
+    return;
+  }
+  const int kept = *count;
+  if (!per_row) {
+    for (int i = tid; i < kept; i += 1024) weight_of[i] = lift;
+    // no kept row: the gradients are zeros
+    if (tid == 0) *gradient_scale = kept == 0 ? 0.f : mean ? *upstream / (float)kept : *upstream;
+    return;
+  }
+  // The largest finite weight is the common scale; infinities and NaN stay with their rows.
+  __shared__ float tops[32];
+  float top = 0.f;
+#pragma unroll 4
+  for (int i = tid; i < kept; i += 1024) {
+    const float g = fabsf(upstream[kept_index[i] * upstream_stride]);
+    if (g <= 3.4028235e38f) top = fmaxf(top, g);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((tid & 31) == 0) tops[tid >> 5] = top;
+  __syncthreads();
+  top = 0.f;
+  for (int w = 0; w < 32; ++w) top = fmaxf(top, tops[w]);
+  if (top == 0.f) top = 1.f;
+  for (int i = tid; i < kept; i += 1024)
+    weight_of[i] = upstream[kept_index[i] * upstream_stride] / top * lift;
+  if (tid == 0) *gradient_scale = top;
+}
+
+}  // namespace attnres_b200

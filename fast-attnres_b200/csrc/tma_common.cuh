@@ -15,7 +15,8 @@
 
 namespace attnres_b200 {
 
-__device__ int g_error_flag = 0;
+// One per translation unit; attnres_b200_error_flag reports them together.
+static __device__ int g_error_flag = 0;
 
 constexpr int kTmaMinWidth = 256;
 constexpr uint64_t kWaitTimeoutNs = 2000000000ull;

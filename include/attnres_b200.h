@@ -40,7 +40,7 @@
 extern "C" {
 #endif
 
-#define ATTNRES_B200_ABI_VERSION 3
+#define ATTNRES_B200_ABI_VERSION 4
 /* Envelope of the reference operator (src/attnres/_sources.py:12-13). */
 #define ATTNRES_B200_MAX_SOURCES 129
 #define ATTNRES_B200_MAX_WIDTH 8192
@@ -59,6 +59,14 @@ extern "C" {
 #define ATTNRES_B200_ERR_BAD_FLAGS 10
 #define ATTNRES_B200_ERR_NOTHING_TO_DO 11     /* backward with neither value nor query gradient */
 #define ATTNRES_B200_ERR_STATIC_SCRATCH 12    /* shape needs more than the built-in dquery scratch */
+
+#define ATTNRES_B200_ERR_BAD_TYPE 13          /* an element type the operator does not take */
+#define ATTNRES_B200_ERR_BAD_VOCABULARY 14    /* vocabulary outside 1..2^25 */
+
+/* Element types of the operators that take more than BF16. */
+#define ATTNRES_B200_BF16 0
+#define ATTNRES_B200_FP16 1
+#define ATTNRES_B200_FP32 2
 
 /* `flags` bits. */
 #define ATTNRES_B200_FLAG_DEFAULT 0u
@@ -293,6 +301,109 @@ int attnres_b200_backward_static_scratch(
     void* const* dsrc_ptrs, const int64_t* dsrc_row_stride,
     void* dq_bf16, float* dq_f32,
     uint32_t flags, void* stream);
+
+/*
+ * The operators at the two ends of a network of reads: LayerNorm, embedding, vocabulary loss.
+ * The reference's model leaves all three to the framework (benchmarks/model.py:156, 239-245 and
+ * its cross entropy in benchmarks/training_graph.py:24-58); there is nothing in it to replace.
+ *
+ * LayerNorm over the last axis as an operator of its own:
+ *   y = (x - mean) * rstd * weight + bias,  rstd = 1/sqrt(var + eps)  (biased variance)
+ *
+ *   x, grad          device [N,D] of `type`, row strides in elements, feature stride 1
+ *   weight, bias     device [D] of `param_type`; NULL means ones / zeros
+ *   y, dx            device [N,D] of `type`, contiguous (dx may be NULL)
+ *   stats            device FP32 [2,N]: mean, then rstd (forward: may be NULL)
+ *   partials         device FP32 workspace [partial_rows, 2 D], partial_rows >=
+ *                    attnres_b200_norm_workspace_rows(N, D, device); only needed with dweight
+ *                    or dbias
+ *   dweight, dbias   device [D] of `param_type`, either may be NULL; summed in a fixed order
+ *
+ * Any width 1..8192, any row stride, any alignment of the element type; 16-byte accesses where
+ * width, strides and addresses allow them.
+ */
+int attnres_b200_norm_forward(
+    const void* x, int64_t x_row_stride, const void* weight, const void* bias, int64_t N, int32_t D,
+    int32_t type, int32_t param_type, float eps, void* y, float* stats, void* stream);
+int32_t attnres_b200_norm_workspace_rows(int64_t N, int32_t D, int32_t device);
+int attnres_b200_norm_backward(
+    const void* grad, int64_t grad_row_stride, const void* x, int64_t x_row_stride,
+    const float* stats, const void* weight, int64_t N, int32_t D, int32_t type, int32_t param_type,
+    void* dx, float* partials, int32_t partial_rows, void* dweight, void* dbias, void* stream);
+
+/*
+ * Embedding: out[n] = scale * table[tokens[n]] + positions[n mod T], summed in FP32, rounded once.
+ *
+ *   tokens           device int64 (`tokens_64` nonzero) or int32 [N], contiguous; N a multiple of T.
+ *                    A row whose id is outside 0..V-1 becomes NaN and has no gradient.
+ *   table, positions device [V,D] / [T,D], own types, row strides in elements, feature stride 1;
+ *                    `positions` may be NULL
+ *   out, grad        device [N,D] of one type; out contiguous, grad with a row stride
+ *   padding_id       id whose row gets no gradient, or -1
+ *   dtable           device [V,D] of `table_type`, contiguous, dense (zeros where no token is);
+ *                    summed in the order of the tokens, the same bits every time; may be NULL
+ *   dpositions       device [T,D] of `position_type`, contiguous; may be NULL
+ *   workspace        16-byte aligned, attnres_b200_embedding_workspace_bytes(N, D) bytes; only
+ *                    needed with dtable
+ */
+int attnres_b200_embedding_forward(
+    const void* tokens, int32_t tokens_64, int64_t N, int64_t T, int32_t V, int32_t D,
+    const void* table, int64_t table_row_stride, int32_t table_type, const void* positions,
+    int64_t position_row_stride, int32_t position_type, float scale, void* out, int32_t out_type,
+    void* stream);
+int64_t attnres_b200_embedding_workspace_bytes(int64_t N, int32_t D);
+int attnres_b200_embedding_backward(
+    const void* tokens, int32_t tokens_64, int64_t N, int64_t T, int32_t V, int32_t D,
+    int64_t padding_id, const void* grad, int64_t grad_row_stride, int32_t grad_type, float scale,
+    void* dtable, int32_t table_type, void* dpositions, int32_t position_type, void* workspace,
+    int64_t workspace_bytes, void* stream);
+
+/*
+ * Softmax cross entropy of scale * hidden @ weight^T, without keeping the logits.
+ *
+ *   hidden           device [N,D], BF16 or FP16 (`type`), row stride in elements, feature stride 1
+ *   weight           device [V,D] of `type`, row stride in elements, feature stride 1
+ *   targets          device int64 (`targets_64` nonzero) or int32 [N].  Rows whose target equals
+ *                    `ignored` take no part: their loss and gradient are zero whatever they hold.
+ *                    Any other target outside 0..V-1 makes its loss and the gradients NaN.
+ *   reduction        ATTNRES_B200_LOSS_NONE, _SUM, _MEAN (over the rows that are not ignored;
+ *                    NaN when there is none)
+ *   losses           device FP32 [N]: the loss of every row
+ *   loss             device FP32 [1]: the reduced loss (unused with _NONE)
+ *
+ * What the backward needs, written by the forward:
+ *   kept             device [N, D rounded up to 8] of `type`, 16-byte aligned: the rows that are
+ *                    not ignored, one behind the other
+ *   kept_index       device int32 [N], their rows in `hidden`
+ *   kept_target      device int32 [N], their targets
+ *   count            device int32 [1], how many there are
+ *   lse2             device FP32 [N]: log2 of each kept row's sum of exponentials
+ *
+ *   upstream         device FP32: [N] with stride `upstream_stride` for _NONE, else one number
+ *   dhidden          device [N,D] of `type`, contiguous; dweight [V,D], contiguous; either may be
+ *                    NULL
+ *   workspace        16-byte aligned, attnres_b200_loss_workspace_bytes(N, V, D, backward) bytes
+ *
+ * The backward forms the logits a second time, a piece of the vocabulary after the other, so
+ * neither pass holds more of [N,V] than one piece (512 MiB, or 4096 ids where that is more).
+ * Results are the same bits every time.
+ */
+#define ATTNRES_B200_LOSS_NONE 0
+#define ATTNRES_B200_LOSS_SUM 1
+#define ATTNRES_B200_LOSS_MEAN 2
+int64_t attnres_b200_loss_workspace_bytes(int64_t N, int32_t V, int32_t D, int32_t backward);
+int attnres_b200_loss_forward(
+    const void* hidden, int64_t hidden_row_stride, const void* weight, int64_t weight_row_stride,
+    const void* targets, int32_t targets_64, int64_t N, int32_t V, int32_t D, int32_t type,
+    int64_t ignored, float scale, int32_t reduction, void* kept, int32_t* kept_index,
+    int32_t* kept_target, int32_t* count, float* lse2, float* losses, float* loss, void* workspace,
+    int64_t workspace_bytes, void* stream);
+int attnres_b200_loss_backward(
+    const float* upstream, int64_t upstream_stride, const void* weight, int64_t weight_row_stride,
+    const void* targets, int32_t targets_64, int64_t N, int32_t V, int32_t D, int32_t type,
+    int64_t ignored, float scale, int32_t reduction, const void* kept, const int32_t* kept_index,
+    const int32_t* kept_target, const int32_t* count, const float* lse2, void* dhidden,
+    void* dweight, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Diagnostics (no counterpart in the reference).  The TMA-staged kernels bound
