@@ -14,6 +14,7 @@ FLAG_FORCE_GENERIC = 1
 FLAG_PREFER_STREAM = 2
 FLAG_ACCUMULATE_DV = 4
 LIBRARY_PATH = Path(__file__).resolve().parent / "_lib" / "libattnres_b200.so"
+OPERATORS_PATH = LIBRARY_PATH.parent / "attnres_b200_torch.so"
 
 _PTR_ARRAY = ctypes.POINTER(c_void_p)
 _I64_ARRAY = ctypes.POINTER(c_int64)
@@ -110,6 +111,17 @@ def load() -> ctypes.CDLL:
         raise RuntimeError(f"libattnres_b200.so has ABI {found}, binding expects {ABI_VERSION}")
     _library = library
     return library
+
+
+def load_operators():
+    """Register the compiled torch operators (LayerNorm, embedding, vocabulary loss) and return
+    their namespace; like the kernels, there is no fallback when they were not built."""
+    import torch
+    load()
+    if not OPERATORS_PATH.exists():
+        raise RuntimeError(f"{OPERATORS_PATH} is missing: run `python fast-attnres_b200/build.py`")
+    torch.ops.load_library(str(OPERATORS_PATH))
+    return torch.ops.attnres_b200
 
 
 def status_text(status: int) -> str:

@@ -10,151 +10,47 @@ positions of a 32 000-word vocabulary); here the logits exist one tile at a time
 """
 from __future__ import annotations
 
-import torch
-from torch.autograd.function import once_differentiable
+import math
 
-from . import _calls, _native, _ops
+import torch
+
+from . import _calls, _native
 from ._sources import MAX_WIDTH, _first_failure, check_scalar
 
-_TYPES = {torch.bfloat16: 0, torch.float16: 1}
+# Compiled operators (csrc/torch_ops.cpp): `linear_cross_entropy_forward` and `..._backward` launch
+# the kernels, `linear_cross_entropy` is the differentiable call over the two.
+_ops = _native.load_operators()
+_linear_cross_entropy = _ops.linear_cross_entropy.default
+_TYPES = _calls.HALVES
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 MAX_ROWS = 1 << 30
 
 
-def _forward(hidden, weight, targets, ignore_index, reduction, scale):
-    """-> (loss, kept rows, their indices, their targets, their count, log2 of their sums)."""
-    width, vocabulary, device = hidden.shape[-1], weight.shape[0], hidden.device
-    rows = hidden.numel() // width
-    kept = torch.empty((rows, (width + 7) // 8 * 8), device=device, dtype=hidden.dtype)
-    index = torch.empty((2, rows), device=device, dtype=torch.int32)
-    count = torch.empty((1,), device=device, dtype=torch.int32)
-    sums = torch.empty((2, rows), device=device, dtype=torch.float32)
-    loss = sums[1] if reduction == 0 else torch.empty((), device=device, dtype=torch.float32)
-    if rows == 0:
-        count.zero_()
-        if reduction != 0:
-            loss.fill_(0.0 if reduction == 1 else float("nan"))
-        return loss.reshape(targets.shape) if reduction == 0 else loss, kept, index, count, sums[0]
-    source, row_stride = _calls.rows_of(hidden)
-    head, head_stride = _calls.rows_of(weight)
-    ids = targets.contiguous()
-    with _calls.on_device(device):
-        size = _native.loss_workspace_bytes(rows, vocabulary, width, False)
-        workspace = torch.empty((size,), device=device, dtype=torch.uint8)
-        _native.loss_forward(
-            source.data_ptr(), row_stride, head.data_ptr(), head_stride, ids.data_ptr(),
-            ids.dtype == torch.int64, rows, vocabulary, width, _TYPES[hidden.dtype], ignore_index,
-            scale, reduction, kept.data_ptr(), index.data_ptr(), index.data_ptr() + 4 * rows,
-            count.data_ptr(), sums.data_ptr(), sums.data_ptr() + 4 * rows, loss.data_ptr(),
-            workspace.data_ptr(), size, _calls.stream(device))
-    return loss.reshape(targets.shape) if reduction == 0 else loss, kept, index, count, sums[0]
+def _loss_like(hidden, targets, reduction):
+    return hidden.new_empty(targets.shape if reduction == 0 else (), dtype=torch.float32)
 
 
-def _backward(grad, weight, targets, kept, index, count, sums, shape, ignore_index, reduction,
-              scale, need_hidden, need_weight):
-    """-> (dhidden, dweight), None where not needed."""
-    width, vocabulary, device = weight.shape[1], weight.shape[0], weight.device
-    rows = targets.numel()
-    dhidden = torch.empty(shape, device=device, dtype=weight.dtype) if need_hidden else None
-    make = torch.empty if rows else torch.zeros
-    dweight = make((vocabulary, width), device=device, dtype=weight.dtype) if need_weight else None
-    if rows == 0 or not (need_hidden or need_weight):
-        return dhidden, dweight
-    head, head_stride = _calls.rows_of(weight)
-    ids = targets.contiguous()
-    upstream = grad.reshape(-1) if grad.is_contiguous() else grad.contiguous().reshape(-1)
-    with _calls.on_device(device):
-        size = _native.loss_workspace_bytes(rows, vocabulary, width, True)
-        workspace = torch.empty((size,), device=device, dtype=torch.uint8)
-        _native.loss_backward(
-            upstream.data_ptr(), 1, head.data_ptr(), head_stride, ids.data_ptr(),
-            ids.dtype == torch.int64, rows, vocabulary, width, _TYPES[weight.dtype], ignore_index,
-            scale, reduction, kept.data_ptr(), index.data_ptr(), index.data_ptr() + 4 * rows,
-            count.data_ptr(), sums.data_ptr(), _calls.pointer(dhidden), _calls.pointer(dweight),
-            workspace.data_ptr(), size, _calls.stream(device))
-    return dhidden, dweight
-
-
-@_ops._custom_op("attnres_b200::linear_cross_entropy_forward", mutates_args=(), device_types="cuda")
-def linear_cross_entropy_forward(
-        hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int,
-        reduction: int, scale: float
-) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """-> (loss, kept rows, [indices, targets] of the kept rows, their count, log2 of their sums)."""
-    loss, kept, index, count, sums = _forward(hidden, weight, targets, ignore_index, reduction, scale)
-    if reduction == 0:
-        loss = loss.clone()   # outputs of an operator do not share storage
-    return loss, kept, index, count, sums.clone()
-
-
-@linear_cross_entropy_forward.register_fake
-def _(hidden, weight, targets, ignore_index, reduction, scale):
+@torch.library.register_fake("attnres_b200::linear_cross_entropy_forward")
+def _(hidden, weight, targets, ignored, reduction, scale):
     width = hidden.shape[-1]
     rows = hidden.numel() // width
-    return (hidden.new_empty(targets.shape if reduction == 0 else (), dtype=torch.float32),
+    return (_loss_like(hidden, targets, reduction),
             hidden.new_empty((rows, (width + 7) // 8 * 8)),
             hidden.new_empty((2, rows), dtype=torch.int32),
             hidden.new_empty((1,), dtype=torch.int32),
             hidden.new_empty((rows,), dtype=torch.float32))
 
 
-@_ops._custom_op("attnres_b200::linear_cross_entropy_backward", mutates_args=(),
-                 device_types="cuda")
-def linear_cross_entropy_backward(
-        grad: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, kept: torch.Tensor,
-        index: torch.Tensor, count: torch.Tensor, sums: torch.Tensor, ignore_index: int,
-        reduction: int, scale: float, need_hidden: bool, need_weight: bool
-) -> tuple[torch.Tensor, torch.Tensor]:
-    """A gradient that is not needed comes back with 0 elements."""
-    dhidden, dweight = _backward(grad, weight, targets, kept, index, count, sums,
-                                 (*targets.shape, weight.shape[1]), ignore_index, reduction, scale,
-                                 need_hidden, need_weight)
-    return (weight.new_empty((0,)) if dhidden is None else dhidden,
-            weight.new_empty((0,)) if dweight is None else dweight)
-
-
-@linear_cross_entropy_backward.register_fake
-def _(grad, weight, targets, kept, index, count, sums, ignore_index, reduction, scale, need_hidden,
+@torch.library.register_fake("attnres_b200::linear_cross_entropy_backward")
+def _(grad, weight, targets, kept, index, count, sums, ignored, reduction, scale, need_hidden,
       need_weight):
     return (weight.new_empty((*targets.shape, weight.shape[1]) if need_hidden else (0,)),
             weight.new_empty(weight.shape if need_weight else (0,)))
 
 
-def _op_setup(ctx, inputs, output) -> None:
-    _hidden, weight, targets, *ctx.constants = inputs
-    ctx.mark_non_differentiable(*output[1:])
-    ctx.set_materialize_grads(False)
-    ctx.save_for_backward(weight, targets, *output[1:])
-
-
-def _op_backward(ctx, grad, *_unused):
-    if grad is None:
-        return (None,) * 6
-    need = bool(ctx.needs_input_grad[0]), bool(ctx.needs_input_grad[1])
-    grads = linear_cross_entropy_backward(grad, *ctx.saved_tensors, *ctx.constants, *need)
-    return (*(g if n else None for g, n in zip(grads, need)), None, None, None, None)
-
-
-torch.library.register_autograd(linear_cross_entropy_forward, _op_backward, setup_context=_op_setup)
-
-
-class _LinearCrossEntropy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, weight, targets, *constants):
-        loss, *kept = _forward(hidden, weight, targets, *constants)
-        ctx.save_for_backward(weight, targets, *kept)
-        ctx.set_materialize_grads(False)
-        ctx.constants, ctx.shape = constants, hidden.shape
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        if grad is None:
-            return (None,) * 6
-        grads = _backward(grad, *ctx.saved_tensors, ctx.shape, *ctx.constants,
-                          *ctx.needs_input_grad[:2])
-        return (*grads, None, None, None, None)
+@torch.library.register_fake("attnres_b200::linear_cross_entropy")
+def _(hidden, weight, targets, ignored, reduction, scale):
+    return _loss_like(hidden, targets, reduction)
 
 
 def _check(hidden, weight, targets, ignore_index, reduction, scale) -> None:
@@ -186,6 +82,19 @@ def _check(hidden, weight, targets, ignore_index, reduction, scale) -> None:
         raise RuntimeError("linear_cross_entropy requires CUDA tensors")
 
 
+def _acceptable(hidden, weight, targets) -> bool:
+    """The conditions of `_check` on the tensors at the cost of a call on a few rows; `_check`
+    names the one that does not hold."""
+    return (isinstance(hidden, torch.Tensor) and isinstance(weight, torch.Tensor)
+            and isinstance(targets, torch.Tensor) and hidden.is_cuda and hidden.dtype in _TYPES
+            and weight.dtype == hidden.dtype and targets.dtype in _calls.INTEGERS
+            and weight.device == hidden.device and targets.device == hidden.device
+            and hidden.ndim > 0 and 1 <= hidden.shape[-1] <= MAX_WIDTH and weight.ndim == 2
+            and weight.shape[1] == hidden.shape[-1]
+            and 1 <= weight.shape[0] <= _calls.MAX_VOCABULARY
+            and targets.shape == hidden.shape[:-1] and targets.numel() <= MAX_ROWS)
+
+
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *,
                          ignore_index: int = -100, reduction: str = "mean",
                          scale: float = 1.0) -> torch.Tensor:
@@ -200,13 +109,10 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     the softmax residue is rounded to the inputs' type before it is multiplied into the gradients,
     which come back in that type.  Differentiable once; results are the same bits every time.
     """
-    _check(hidden, weight, targets, ignore_index, reduction, scale)
-    constants = ignore_index, _REDUCTIONS[reduction], float(scale)
-    if not _calls.direct(hidden, weight, targets):
-        return linear_cross_entropy_forward(hidden, weight, targets, *constants)[0]
-    if _calls.wants_grad(hidden, weight):
-        return _LinearCrossEntropy.apply(hidden, weight, targets, *constants)
-    return _forward(hidden, weight, targets, *constants)[0]
+    if not (_acceptable(hidden, weight, targets) and type(ignore_index) is int
+            and reduction in _REDUCTIONS and _calls.plain_number(scale) and math.isfinite(scale)):
+        _check(hidden, weight, targets, ignore_index, reduction, scale)
+    return _linear_cross_entropy(hidden, weight, targets, ignore_index, _REDUCTIONS[reduction], scale)
 
 
 __all__ = ["linear_cross_entropy"]

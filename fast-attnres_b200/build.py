@@ -1,8 +1,10 @@
 """Build the sm_100a shared library in-tree: ``python fast-attnres_b200/build.py``.
 
-One ``nvcc`` invocation compiles the translation units of ``csrc`` (the read, LayerNorm,
-embedding and the vocabulary loss; each includes its kernel headers), side by side, into ``attnres/_lib/libattnres_b200.so``.  nvcc cross-compiles
-for sm_100a, so no GPU is needed to build.
+``nvcc`` compiles the translation units of ``csrc`` side by side (the read, LayerNorm, embedding
+and the vocabulary loss; a unit is compiled again when it or a header it includes is newer than
+its object file) and links them into ``attnres/_lib/libattnres_b200.so``; ``g++`` builds the torch
+operators over its C ABI (``csrc/torch_ops.cpp``) into ``attnres/_lib/attnres_b200_torch.so``.  nvcc
+cross-compiles for sm_100a, so no GPU is needed to build.
 """
 from __future__ import annotations
 
@@ -18,6 +20,8 @@ ROOT = Path(__file__).resolve().parent
 SOURCES = [ROOT / "csrc" / name for name in ("attnres_b200.cu", "norm.cu", "embedding.cu", "loss.cu")]
 HEADERS = sorted((ROOT / "csrc").glob("*.cuh")) + [ROOT.parent / "include" / "attnres_b200.h"]
 OUTPUT = ROOT / "attnres" / "_lib" / "libattnres_b200.so"
+OPERATORS = ROOT / "csrc" / "torch_ops.cpp"
+OPERATORS_OUTPUT = ROOT / "attnres" / "_lib" / "attnres_b200_torch.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -67,13 +71,32 @@ def _run(command: list[str]) -> str:
     result = subprocess.run(command, capture_output=True, text=True)
     if result.returncode != 0:
         sys.stderr.write(result.stdout + result.stderr)
-        raise RuntimeError(f"nvcc failed with exit code {result.returncode}")
+        raise RuntimeError(f"{command[0]} failed with exit code {result.returncode}")
     return result.stdout + result.stderr
+
+
+def _build_operators(force: bool) -> Path:
+    """The torch operators over the C ABI: host code only, linked against the kernel library."""
+    import torch
+    from torch.utils import cpp_extension
+    newest = max(path.stat().st_mtime for path in [*_includes(OPERATORS, set()), Path(__file__)])
+    if not force and OPERATORS_OUTPUT.exists() and newest <= OPERATORS_OUTPUT.stat().st_mtime:
+        return OPERATORS_OUTPUT
+    cuda = Path(_nvcc()).resolve().parents[1]
+    libraries = cpp_extension.library_paths()
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          *(f"-isystem{path}" for path in [*cpp_extension.include_paths(), cuda / "include"]),
+          str(OPERATORS), *(f"-L{path}" for path in [*libraries, OUTPUT.parent]),
+          "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", f"-l:{OUTPUT.name}",
+          "-Wl,-rpath,$ORIGIN", "-o", str(OPERATORS_OUTPUT)])
+    return OPERATORS_OUTPUT
 
 
 def build(*, force: bool = False, verbose: bool = False) -> Path:
     """Compile the library if any source is newer than it; return its path."""
     if not force and up_to_date():
+        _build_operators(force)
         return OUTPUT
     OUTPUT.parent.mkdir(parents=True, exist_ok=True)
     with ThreadPoolExecutor(len(SOURCES)) as pool:
@@ -82,6 +105,7 @@ def build(*, force: bool = False, verbose: bool = False) -> Path:
         sys.stderr.write("".join(text for _, text in compiled))
     _run([_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-shared",
           *(str(target) for target, _ in compiled), "-o", str(OUTPUT)])
+    _build_operators(force)
     return OUTPUT
 
 
