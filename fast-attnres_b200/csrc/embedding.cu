@@ -8,7 +8,7 @@ namespace attnres_b200 {
 namespace {
 
 constexpr int64_t kMaxTokens = (1ll << 31) - 1;  // positions are 32-bit inside the sort
-constexpr int32_t kMaxVocabulary = 1 << 25;      // the helpers' bitmaps hold a range each
+constexpr int32_t kMaxVocabulary = 1 << 25;
 
 int check_embedding(int64_t N, int64_t T, int32_t V, int32_t D, int32_t type, int32_t out_type,
                     int32_t position_type, float scale) {
@@ -27,6 +27,72 @@ int64_t tile_pairs(int64_t N) {
   // joining of one very frequent id stay bounded (4096 tiles).
   const int64_t grown = (N + 4095) / 4096;
   return grown <= 32 ? 32 : (grown + 7) / 8 * 8;
+}
+
+template <bool VECTOR, bool WIDE>
+int launch_embedding_forward(const EmbedParams& p, int lanes, dim3 grid, cudaStream_t stream) {
+  if (p.positions == nullptr)
+    embedding_fwd_kernel<VECTOR, WIDE, kNoPositions><<<grid, kEmbedThreads, 0, stream>>>(p, lanes);
+  else if (p.position_type != ATTNRES_B200_FP32)
+    embedding_fwd_kernel<VECTOR, WIDE, kNarrowPositions><<<grid, kEmbedThreads, 0, stream>>>(p, lanes);
+  else
+    embedding_fwd_kernel<VECTOR, WIDE, kWidePositions><<<grid, kEmbedThreads, 0, stream>>>(p, lanes);
+  return launched();
+}
+
+// A launch that may start before the kernel in front of it has ended (that kernel says when).
+template <typename... Parameters, typename... Arguments>
+int launch_beside(void (*kernel)(Parameters...), int64_t grid, int threads, bool beside,
+                  cudaStream_t stream, Arguments... arguments) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)grid);
+  config.blockDim = dim3((unsigned)threads);
+  config.stream = stream;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = beside ? 1 : 0;
+  if (cudaLaunchKernelEx(&config, kernel, Parameters(arguments)...) != cudaSuccess) {
+    cudaGetLastError();
+    return ATTNRES_B200_ERR_CUDA;
+  }
+  return ATTNRES_B200_OK;
+}
+
+template <bool VECTOR, bool WIDE>
+int launch_embedding_backward(const EmbedParams& p, int sms, cudaStream_t cs) {
+  static SmemGrant grant;
+  int64_t fill_ctas = 0, position_ctas = 0;
+  if (p.dtable != nullptr) {
+    if (int st = prepare_kernel(embedding_sort_kernel, kSortSmem, grant)) return st;
+    embedding_sort_kernel<<<kSortCluster, kSortThreads, kSortSmem, cs>>>(p);
+    if (int st = launched()) return st;
+    // Every filling CTA reads all ids: few of them where that takes longer than the filling.
+    fill_ctas = p.N <= 65536 ? 4 * sms : sms;
+    const int64_t ranges = ((int64_t)p.V + kFillRange - 2) / (kFillRange - 1);
+    if (fill_ctas < ranges) fill_ctas = ranges;  // a bitmap holds its CTA's range
+    if (fill_ctas > p.V) fill_ctas = p.V;
+  }
+  if (p.dpositions != nullptr)
+    position_ctas = (p.T * ((p.D + 7) / 8) + kEarlyThreads - 1) / kEarlyThreads;
+  if (int st = launch_beside(embedding_early_kernel<VECTOR, WIDE>, fill_ctas + position_ctas,
+                             kEarlyThreads, p.dtable != nullptr, cs, p, type_bytes(p.table_type),
+                             (int)fill_ctas))
+    return st;
+  if (p.dtable == nullptr) return ATTNRES_B200_OK;
+  const int64_t tiles = (p.N + p.tile - 1) / p.tile;
+  const auto [lanes, blocks] = columns_of(p.D, gradient_columns<VECTOR>());
+  const int64_t units = tiles * blocks;
+  const int per_cta = kEmbedThreads / lanes;
+  embedding_sum_kernel<VECTOR, WIDE>
+      <<<(unsigned)((units + per_cta - 1) / per_cta), kEmbedThreads, 0, cs>>>(p, lanes, blocks, tiles);
+  if (int st = launched()) return st;
+  if (tiles == 1) return ATTNRES_B200_OK;
+  constexpr int warps = kEmbedThreads / 32;
+  const int64_t joins = (units + warps - 1) / warps;
+  return launch_beside(embedding_join_kernel<VECTOR>, joins < 2 * sms ? joins : 2 * sms,
+                       kEmbedThreads, true, cs, p, lanes, blocks, tiles);
 }
 
 int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -66,20 +132,24 @@ extern "C" int attnres_b200_embedding_forward(
   const bool vector = D % 8 == 0 && aligned16(table) && table_row_stride % 8 == 0 &&
                       aligned16(out) &&
                       (!positions || (aligned16(positions) && position_row_stride % 8 == 0));
-  const int lanes = embed_lanes(D), rows = kEmbedThreads / lanes;
-  const int columns = lanes * 8 * kEmbedBlocks;
-  const dim3 grid((unsigned)((N + rows - 1) / rows), (unsigned)((D + columns - 1) / columns));
+  const auto [lanes, blocks] = columns_of(D, 8);
+  const int rows = kEmbedThreads / lanes;
+  const dim3 grid((unsigned)((N + rows - 1) / rows),
+                  (unsigned)((blocks + kEmbedBlocks - 1) / kEmbedBlocks));
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  if (vector) embedding_fwd_kernel<true><<<grid, kEmbedThreads, 0, cs>>>(p, lanes);
-  else embedding_fwd_kernel<false><<<grid, kEmbedThreads, 0, cs>>>(p, lanes);
-  return launched();
+  if (table_type == ATTNRES_B200_FP32)
+    return vector ? launch_embedding_forward<true, true>(p, lanes, grid, cs)
+                  : launch_embedding_forward<false, true>(p, lanes, grid, cs);
+  return vector ? launch_embedding_forward<true, false>(p, lanes, grid, cs)
+                : launch_embedding_forward<false, false>(p, lanes, grid, cs);
 }
 
 extern "C" int64_t attnres_b200_embedding_workspace_bytes(int64_t N, int32_t D) {
   if (D < 1 || D > kMaxWidth) return -ATTNRES_B200_ERR_BAD_WIDTH;
   if (N < 1 || N > kMaxTokens) return -ATTNRES_B200_ERR_BAD_ROWS;
   const int64_t tile = tile_pairs(N), tiles = (N + tile - 1) / tile;
-  return 2 * align256(N * (int64_t)sizeof(uint2)) + tiles * 2 * D * (int64_t)sizeof(float);
+  return 2 * align256(N * (int64_t)sizeof(uint2)) + align256((tiles + 1) * (int64_t)sizeof(int32_t)) +
+         tiles * 2 * D * (int64_t)sizeof(float);
 }
 
 extern "C" int attnres_b200_embedding_backward(
@@ -118,42 +188,21 @@ extern "C" int attnres_b200_embedding_backward(
   p.pairs[0] = static_cast<uint2*>(workspace);
   p.pairs[1] = reinterpret_cast<uint2*>(static_cast<char*>(workspace) +
                                         align256(N * (int64_t)sizeof(uint2)));
-  p.pieces = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                      2 * align256(N * (int64_t)sizeof(uint2)));
+  p.tile = (int32_t)tile_pairs(N);
+  const int64_t tiles = (N + p.tile - 1) / p.tile;
+  char* rest = static_cast<char*>(workspace) + 2 * align256(N * (int64_t)sizeof(uint2));
+  p.runs = reinterpret_cast<int32_t*>(rest);
+  p.pieces = reinterpret_cast<float*>(rest + align256((tiles + 1) * (int64_t)sizeof(int32_t)));
   int bits = 1;  // of the ids and of V itself, which marks a token without a gradient
   while ((V >> bits) != 0) ++bits;
   p.passes = (bits + kSortMaxDigitBits - 1) / kSortMaxDigitBits;
   p.digit_bits = (bits + p.passes - 1) / p.passes;
-  const int64_t tile = tile_pairs(N), tiles = (N + tile - 1) / tile;
-  p.tile = (int32_t)tile;
   const bool vector = D % 8 == 0 && aligned16(grad) && (N == 1 || grad_row_stride % 8 == 0) &&
                       (!dtable || aligned16(dtable)) && (!dpositions || aligned16(dpositions));
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  // One CTA per SM: the first cluster sorts, the others write zero rows and position gradients.
-  const int clusters = sms >= 2 * kSortCluster ? sms / kSortCluster : 2;
-  // Reached on a device with few SMs only (a slice of a GPU): a bitmap would not hold its range.
-  if ((int64_t)(clusters - 1) * kSortCluster * (kSortMaxRange - 1) < (int64_t)V)
-    return ATTNRES_B200_ERR_BAD_VOCABULARY;
-  static SmemGrant grant_vector, grant_scalar;
-  if (vector) {
-    if (int st = prepare_kernel(embedding_sort_kernel<true>, kSortSmem, grant_vector)) return st;
-    embedding_sort_kernel<true><<<clusters * kSortCluster, kSortThreads, kSortSmem, cs>>>(
-        p, type_bytes(table_type));
-  } else {
-    if (int st = prepare_kernel(embedding_sort_kernel<false>, kSortSmem, grant_scalar)) return st;
-    embedding_sort_kernel<false><<<clusters * kSortCluster, kSortThreads, kSortSmem, cs>>>(
-        p, type_bytes(table_type));
-  }
-  if (int st = launched()) return st;
-  if (!dtable) return ATTNRES_B200_OK;
-  const int lanes = embed_lanes(D), blocks = (D + lanes * 8 - 1) / (lanes * 8);
-  const int units = kEmbedThreads / lanes;
-  const unsigned grid = (unsigned)((tiles * blocks + units - 1) / units);
-  if (vector) embedding_sum_kernel<true><<<grid, kEmbedThreads, 0, cs>>>(p, lanes, blocks, tiles);
-  else embedding_sum_kernel<false><<<grid, kEmbedThreads, 0, cs>>>(p, lanes, blocks, tiles);
-  if (int st = launched()) return st;
-  if (tiles == 1) return ATTNRES_B200_OK;
-  if (vector) embedding_join_kernel<true><<<grid, kEmbedThreads, 0, cs>>>(p, lanes, blocks, tiles);
-  else embedding_join_kernel<false><<<grid, kEmbedThreads, 0, cs>>>(p, lanes, blocks, tiles);
-  return launched();
+  if (grad_type == ATTNRES_B200_FP32)
+    return vector ? launch_embedding_backward<true, true>(p, sms, cs)
+                  : launch_embedding_backward<false, true>(p, sms, cs);
+  return vector ? launch_embedding_backward<true, false>(p, sms, cs)
+                : launch_embedding_backward<false, false>(p, sms, cs);
 }

@@ -7,9 +7,10 @@
 // Sums are FP32 and are rounded once.  The table's gradient is dense, so its cost is the write of
 // [V, D] plus the read of [N, D].  It is formed in a fixed order without atomics on values:
 //
-//  1. embedding_sort_kernel: one cluster sorts the pairs (id, position) by id, stable, while all
-//     other clusters write the zero rows of ids that do not occur (each reads the ids itself and
-//     marks those of its own range, so nobody waits for the sort) and sum the position gradient.
+//  1. embedding_sort_kernel: one cluster sorts the pairs (id, position) by id, stable.  Beside it
+//     runs embedding_early_kernel with what needs nothing of the sort: the zero rows of ids that do
+//     not occur (its CTAs read the ids themselves and mark those of their own range) and the
+//     position gradient.
 //  2. embedding_sum_kernel: tiles of consecutive sorted pairs; a run of equal ids that lies inside
 //     a tile is summed and stored, the pieces of a run that crosses tiles go to a workspace.  The
 //     load does not depend on how skewed the ids are.
@@ -48,6 +49,7 @@ struct EmbedParams {
   int32_t passes, digit_bits;
   int32_t tile;      // sorted pairs of a tile
   float* pieces;     // [tiles][2][D]: leading and trailing run of a tile
+  int32_t* runs;     // how many runs cross tiles, then the tiles they begin in
 };
 
 __device__ __forceinline__ int64_t load_id(const EmbedParams& p, int64_t n) {
@@ -61,70 +63,86 @@ __device__ __forceinline__ uint32_t gradient_key(const EmbedParams& p, int64_t n
   return (id < 0 || id >= p.V || id == p.padding) ? (uint32_t)p.V : (uint32_t)id;
 }
 
-// Lanes that share one row (a power of two): a warp serves 32 / lanes narrow rows at once.
-inline int embed_lanes(int D) {
-  int lanes = 1;
-  while (lanes < 32 && lanes * 8 < D) lanes *= 2;
-  return lanes;
+// What a lane owns of a block of columns: eight neighbours where rows allow 16-byte accesses, else
+// `elements` of them `lanes` apart.
+struct Columns {
+  int lanes;   // that share one row (a power of two); a warp serves 32 / lanes narrow rows at once
+  int blocks;  // of lanes * elements columns
+};
+
+inline Columns columns_of(int D, int elements) {
+  Columns c{1, 0};
+  while (c.lanes < 32 && c.lanes * elements < D) c.lanes *= 2;
+  c.blocks = (D + c.lanes * elements - 1) / (c.lanes * elements);
+  return c;
 }
 
-// What a lane owns of a block of 8 * lanes columns.
-template <bool VECTOR>
+template <bool VECTOR, int E>
 __device__ __forceinline__ int first_column(int block, int lanes, int lane) {
-  return VECTOR ? (block * lanes + lane) * 8 : block * lanes * 8 + lane;
+  return VECTOR ? (block * lanes + lane) * 8 : block * lanes * E + lane;
 }
-template <bool VECTOR>
+template <bool VECTOR, int E>
 __device__ __forceinline__ int owned_columns(int column, int lanes, int D) {
   if (column >= D) return 0;
   if constexpr (VECTOR) return 8;
-  return min(8, (D - column + lanes - 1) / lanes);
+  int count = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) count += column + e * lanes < D;
+  return count;
 }
 
 constexpr int kEmbedThreads = 256;
 constexpr int kEmbedBlocks = 4;  // column blocks of one forward unit
 
+// Columns a lane of the gradient's kernels owns.  A warp sums a tile of 32 pairs in one block of
+// columns, one row after the other; element by element eight columns would leave too few warps and
+// too many instructions to each (6185 ids of 1001 columns: 38 us with eight, MEASURE with two).
 template <bool VECTOR>
+__host__ __device__ constexpr int gradient_columns() {
+  return VECTOR ? 8 : 2;
+}
+
+enum EmbedPositions { kNoPositions, kNarrowPositions, kWidePositions };
+
+template <bool VECTOR, bool WIDE, int POSITIONS>
 __global__ void __launch_bounds__(kEmbedThreads)
 embedding_fwd_kernel(const EmbedParams p, int lanes) {
+  constexpr bool kAdd = POSITIONS != kNoPositions, kAddWide = POSITIONS == kWidePositions;
   const int lane = threadIdx.x % lanes;
   const int64_t n = (int64_t)blockIdx.x * (kEmbedThreads / lanes) + threadIdx.x / lanes;
   if (n >= p.N) return;
   const int64_t id = load_id(p, n);
   const bool known = id >= 0 && id < p.V;
   const int64_t row = known ? id * p.table_row_stride : 0;
-  const int64_t position = p.positions != nullptr ? (n % p.T) * p.position_row_stride : 0;
-  Raw8 raw[kEmbedBlocks], add[kEmbedBlocks];
+  const int64_t position = kAdd ? (n % p.T) * p.position_row_stride : 0;
+  Share<VECTOR, WIDE> raw[kEmbedBlocks];
+  Share<VECTOR, kAddWide> add[kAdd ? kEmbedBlocks : 1];
 #pragma unroll
   for (int b = 0; b < kEmbedBlocks; ++b) {
-    const int column = first_column<VECTOR>(blockIdx.y * kEmbedBlocks + b, lanes, lane);
-    const int count = owned_columns<VECTOR>(column, lanes, p.D);
+    const int column = first_column<VECTOR, 8>(blockIdx.y * kEmbedBlocks + b, lanes, lane);
+    const int count = owned_columns<VECTOR, 8>(column, lanes, p.D);
     if (count > 0) {
-      if (known) raw[b] = load_raw8<VECTOR>(p.table, p.table_type, row + column, lanes, count);
-      if (p.positions != nullptr)
-        add[b] = load_raw8<VECTOR>(p.positions, p.position_type, position + column, lanes, count);
+      raw[b].load(p.table, row + column, lanes, count);
+      if constexpr (kAdd) add[b].load(p.positions, position + column, lanes, count);
     }
   }
 #pragma unroll
   for (int b = 0; b < kEmbedBlocks; ++b) {
-    const int column = first_column<VECTOR>(blockIdx.y * kEmbedBlocks + b, lanes, lane);
-    const int count = owned_columns<VECTOR>(column, lanes, p.D);
+    const int column = first_column<VECTOR, 8>(blockIdx.y * kEmbedBlocks + b, lanes, lane);
+    const int count = owned_columns<VECTOR, 8>(column, lanes, p.D);
     if (count > 0) {
       float f[8], q[8];
-      if (known) {
-        unpack_raw8(raw[b], p.table_type, f);
+      raw[b].unpack(p.table_type, f);
+      // No such row (row 0 was read in its place): not a number, so that a wrong id cannot pass
+      // unseen.
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= p.scale;
-      } else {
-        // No such row: not a number, so that a wrong id cannot pass unseen.
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = __int_as_float(0x7fc00000);
-      }
-      if (p.positions != nullptr) {
-        unpack_raw8(add[b], p.position_type, q);
+      for (int e = 0; e < 8; ++e) f[e] = known ? f[e] * p.scale : __int_as_float(0x7fc00000);
+      if constexpr (kAdd) {
+        add[b].unpack(p.position_type, q);
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] += q[e];
       }
-      store8<VECTOR>(p.out, p.out_type, n * p.D + column, lanes, count, f);
+      store_share<VECTOR>(p.out, p.out_type, n * p.D + column, lanes, count, f);
     }
   }
 }
@@ -136,14 +154,17 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortMaxDigitBits = 9;
 constexpr int kSortDigits = 1 << kSortMaxDigitBits;
-// Per-warp digit counts, the CTA's totals and the digits' first places; the other clusters use
-// the same bytes as the bitmap of their range of ids.
+// Per-warp digit counts, the CTA's totals and the digits' first places.
 constexpr uint32_t kSortSmem = (kSortWarps + 2) * kSortDigits * 4 + 64;
-constexpr int kSortMaxRange = (int)(kSortSmem - 64) * 8;  // ids a bitmap holds
 
 // Stable radix sort of (id, position) by one cluster.  Every warp owns a contiguous share of the
 // sequence; a digit's places are ordered by warp, and inside a warp by sequence order.
-__device__ inline void sort_pairs(const EmbedParams& p, uint32_t* smem) {
+__global__ void __cluster_dims__(kSortCluster, 1, 1) __launch_bounds__(kSortThreads, 1)
+embedding_sort_kernel(const EmbedParams p) {
+  // The kernel beside this one may start at once; it waits for this one before it ends.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ uint32_t smem[];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.runs = 0;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -238,98 +259,118 @@ __device__ __forceinline__ void zero_row(char* row, int64_t bytes, int lane) {
   for (int64_t i = tail + lane * 2; i < bytes; i += 64) *reinterpret_cast<unsigned short*>(row + i) = 0;
 }
 
-template <bool VECTOR>
-__global__ void __cluster_dims__(kSortCluster, 1, 1) __launch_bounds__(kSortThreads, 1)
-embedding_sort_kernel(const EmbedParams p, int element_bytes) {
-  extern __shared__ uint32_t sort_smem[];
+constexpr int kFillWords = 1024;  // bitmap of the ids a CTA fills
+constexpr int kFillRange = kFillWords * 32;
+
+constexpr int kPositionBatch = 4;  // sequences whose rows a thread has in flight
+constexpr int kEarlyThreads = 256;
+
+// CTAs [0, fill_ctas) write the zero rows of a range of ids each, the others the position gradient.
+template <bool VECTOR, bool WIDE>
+__global__ void __launch_bounds__(kEarlyThreads, VECTOR ? 5 : 3)
+embedding_early_kernel(const EmbedParams p, int element_bytes, int fill_ctas) {
+  __shared__ uint32_t used[kFillWords];
   const int tid = threadIdx.x;
-  if (blockIdx.x < kSortCluster) {
-    if (p.dtable != nullptr) sort_pairs(p, sort_smem);
-    return;
-  }
-  const int helper = blockIdx.x - kSortCluster, helpers = gridDim.x - kSortCluster;
-  if (p.dpositions != nullptr) {
+  if ((int)blockIdx.x < fill_ctas) {
+    // Ids [low, low + range) are this CTA's; a bit is set for those that have a gradient.
+    const int64_t low = (int64_t)p.V * blockIdx.x / fill_ctas;
+    const int range = (int)((int64_t)p.V * (blockIdx.x + 1) / fill_ctas - low);
+    for (int i = tid; i < (range + 31) / 32; i += kEarlyThreads) used[i] = 0u;
+    __syncthreads();
+#pragma unroll 8
+    for (int64_t n = tid; n < p.N; n += kEarlyThreads) {
+      const int64_t key = (int64_t)gradient_key(p, n) - low;
+      if (key >= 0 && key < range) atomicOr(&used[key >> 5], 1u << (key & 31));
+    }
+    __syncthreads();
+    const int64_t row_bytes = (int64_t)p.D * element_bytes;
+    for (int v = tid >> 5; v < range; v += kEarlyThreads / 32) {
+      if (!((used[v >> 5] >> (v & 31)) & 1u))
+        zero_row(static_cast<char*>(p.dtable) + (low + v) * row_bytes, row_bytes, tid & 31);
+    }
+  } else {
     const int chunks = (p.D + 7) / 8;
     const int64_t items = p.T * chunks, batch = p.N / p.T;
-    for (int64_t i = (int64_t)helper * kSortThreads + tid; i < items;
-         i += (int64_t)helpers * kSortThreads) {
+    const int64_t i = (int64_t)(blockIdx.x - fill_ctas) * kEarlyThreads + tid;
+    if (i < items) {
       const int64_t t = i / chunks;
-      const int column = (int)(i % chunks) * 8, count = min(8, p.D - column);
+      const int column = (int)(i - t * chunks) * 8, count = min(8, p.D - column);
       float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (int64_t b = 0; b < batch; ++b) {
-        float f[8];
-        unpack_raw8(load_raw8<VECTOR>(p.grad, p.out_type,
-                                      (b * p.T + t) * p.grad_row_stride + column, 1, count),
-                    p.out_type, f);
+      for (int64_t b = 0; b < batch; b += kPositionBatch) {
+        Share<VECTOR, WIDE> raw[kPositionBatch];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] += f[e];
+        for (int k = 0; k < kPositionBatch; ++k)
+          if (b + k < batch)
+            raw[k].load(p.grad, ((b + k) * p.T + t) * p.grad_row_stride + column, 1, count);
+#pragma unroll
+        for (int k = 0; k < kPositionBatch; ++k) {
+          if (b + k < batch) {
+            float f[8];
+            raw[k].unpack(p.out_type, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] += f[e];
+          }
+        }
       }
-      store8<VECTOR>(p.dpositions, p.position_type, t * p.D + column, 1, count, sum);
+      store_share<VECTOR>(p.dpositions, p.position_type, t * p.D + column, 1, count, sum);
     }
   }
-  if (p.dtable == nullptr) return;
-  // Ids [low, high) are this CTA's; a bit is set for those that have a gradient.
-  const int64_t low = (int64_t)p.V * helper / helpers, high = (int64_t)p.V * (helper + 1) / helpers;
-  const int range = (int)(high - low), words = (range + 31) / 32;
-  for (int i = tid; i < words; i += kSortThreads) sort_smem[i] = 0u;
-  __syncthreads();
-#pragma unroll 4
-  for (int64_t n = tid; n < p.N; n += kSortThreads) {
-    const int64_t key = (int64_t)gradient_key(p, n) - low;
-    if (key >= 0 && key < range) atomicOr(&sort_smem[key >> 5], 1u << (key & 31));
-  }
-  __syncthreads();
-  const int64_t row_bytes = (int64_t)p.D * element_bytes;
-  for (int v = tid >> 5; v < range; v += kSortWarps) {
-    if (!((sort_smem[v >> 5] >> (v & 31)) & 1u))
-      zero_row(static_cast<char*>(p.dtable) + (low + v) * row_bytes, row_bytes, tid & 31);
-  }
+  // What follows in the stream waits for this kernel, and through this also for the sort.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ------------------------------------------------------------------------------ gradient, step 2
 
-constexpr int kSumBatch = 8;  // rows in flight per lane
+constexpr int kJoinBatch = 8;  // pieces in flight per lane
 
-template <bool VECTOR>
+template <bool VECTOR, bool WIDE>
 __global__ void __launch_bounds__(kEmbedThreads)
 embedding_sum_kernel(const EmbedParams p, int lanes, int blocks, int64_t tiles) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining waits for the end
+  constexpr int E = gradient_columns<VECTOR>();
+  constexpr int kSumBatch = VECTOR ? 8 : 16;  // rows in flight per lane
   const int lane = threadIdx.x % lanes;
   const int64_t unit = (int64_t)blockIdx.x * (kEmbedThreads / lanes) + threadIdx.x / lanes;
   const int64_t tile = unit / blocks;
-  const int column = first_column<VECTOR>((int)(unit % blocks), lanes, lane);
-  const int count = owned_columns<VECTOR>(column, lanes, p.D);
+  const int column = first_column<VECTOR, E>((int)(unit % blocks), lanes, lane);
+  const int count = owned_columns<VECTOR, E>(column, lanes, p.D);
   if (tile >= tiles || count == 0) return;
   const uint2* pairs = p.pairs[(p.passes - 1) & 1];
   const uint32_t nothing = (uint32_t)p.V;
   const int64_t begin = tile * p.tile, end = min(p.N, begin + p.tile);
   const uint32_t before = begin > 0 ? __ldg(&pairs[begin - 1].x) : nothing;
   const uint32_t after = end < p.N ? __ldg(&pairs[end].x) : nothing;
-  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float sum[E] = {};
   uint32_t current = __ldg(&pairs[begin].x);
   bool leading = current == before;  // the run began in an earlier tile
   auto finish = [&](bool continues) {
     if (current == nothing) return;
     if (!leading && !continues) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] *= p.scale;
-      store8<VECTOR>(p.dtable, p.table_type, (int64_t)current * p.D + column, lanes, count, sum);
+      for (int e = 0; e < E; ++e) sum[e] *= p.scale;
+      store_share<VECTOR, E>(p.dtable, p.table_type, (int64_t)current * p.D + column, lanes, count, sum);
     } else {
-      store8<VECTOR>(p.pieces, ATTNRES_B200_FP32, (2 * tile + (leading ? 0 : 1)) * p.D + column,
+      store_share<VECTOR, E>(p.pieces, ATTNRES_B200_FP32, (2 * tile + (leading ? 0 : 1)) * p.D + column,
                      lanes, count, sum);
     }
   };
-  for (int64_t i = begin; i < end; i += kSumBatch) {
-    uint2 pair[kSumBatch];
-    Raw8 raw[kSumBatch];
+  uint2 next[kSumBatch];
+  auto fetch = [&](int64_t i) {
 #pragma unroll
     for (int k = 0; k < kSumBatch; ++k)
-      pair[k] = i + k < end ? __ldg(pairs + i + k) : make_uint2(nothing, 0u);
+      next[k] = i + k < end ? __ldg(pairs + i + k) : make_uint2(nothing, 0u);
+  };
+  fetch(begin);
+  for (int64_t i = begin; i < end; i += kSumBatch) {
+    uint2 pair[kSumBatch];
+    Share<VECTOR, WIDE, E> raw[kSumBatch];
+#pragma unroll
+    for (int k = 0; k < kSumBatch; ++k) pair[k] = next[k];
 #pragma unroll
     for (int k = 0; k < kSumBatch; ++k)
       if (pair[k].x != nothing)
-        raw[k] = load_raw8<VECTOR>(p.grad, p.out_type,
-                                   (int64_t)pair[k].y * p.grad_row_stride + column, lanes, count);
+        raw[k].load(p.grad, (int64_t)pair[k].y * p.grad_row_stride + column, lanes, count);
+    fetch(i + kSumBatch);
 #pragma unroll
     for (int k = 0; k < kSumBatch; ++k) {
       if (i + k < end) {
@@ -338,67 +379,72 @@ embedding_sum_kernel(const EmbedParams p, int lanes, int blocks, int64_t tiles) 
           current = pair[k].x;
           leading = false;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+          for (int e = 0; e < E; ++e) sum[e] = 0.f;
         }
         if (current != nothing) {
-          float f[8];
-          unpack_raw8(raw[k], p.out_type, f);
+          float f[E];
+          raw[k].unpack(p.out_type, f);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sum[e] += f[e];
+          for (int e = 0; e < E; ++e) sum[e] += f[e];
         }
       }
     }
   }
-  finish(current == after);
+  const bool continues = current == after && current != nothing;
+  finish(continues);
+  // A run that begins here and goes on: one of the kernel's units puts it on the list to join.
+  if (continues && !leading && column == 0) p.runs[1 + atomicAdd(p.runs, 1)] = (int32_t)tile;
 }
 
 // ------------------------------------------------------------------------------ gradient, step 3
 
+// A warp joins the pieces of one run in one block of columns.  (The order of the list is not fixed,
+// but each run is joined on its own, in tile order.)
 template <bool VECTOR>
 __global__ void __launch_bounds__(kEmbedThreads)
 embedding_join_kernel(const EmbedParams p, int lanes, int blocks, int64_t tiles) {
-  const int lane = threadIdx.x % lanes;
-  const int64_t unit = (int64_t)blockIdx.x * (kEmbedThreads / lanes) + threadIdx.x / lanes;
-  const int64_t tile = unit / blocks;
-  const int column = first_column<VECTOR>((int)(unit % blocks), lanes, lane);
-  const int count = owned_columns<VECTOR>(column, lanes, p.D);
-  if (tile >= tiles - 1 || count == 0) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr int E = gradient_columns<VECTOR>();
+  const int lane = threadIdx.x & 31;
   const uint2* pairs = p.pairs[(p.passes - 1) & 1];
-  const int64_t begin = tile * p.tile, end = begin + p.tile;  // a tile follows, so this one is full
-  const uint32_t id = __ldg(&pairs[end - 1].x);
-  if (id == (uint32_t)p.V || __ldg(&pairs[end].x) != id) return;
-  // Only the tile in which the run begins joins it.
-  if (begin > 0 && __ldg(&pairs[begin].x) == id && __ldg(&pairs[begin - 1].x) == id) return;
-  float sum[8], f[8];
-  unpack_raw8(load_raw8<VECTOR>(p.pieces, ATTNRES_B200_FP32, (2 * tile + 1) * p.D + column, lanes,
-                                count),
-              ATTNRES_B200_FP32, sum);
-  int64_t next = tile + 1;
-  while (next < tiles) {
-    bool in_run[4];
-    Raw8 raw[4];
+  const int64_t units = (int64_t)__ldcg(p.runs) * blocks;
+  for (int64_t unit = (int64_t)blockIdx.x * (kEmbedThreads / 32) + threadIdx.x / 32; unit < units;
+       unit += (int64_t)gridDim.x * (kEmbedThreads / 32)) {
+    const int64_t tile = __ldcg(p.runs + 1 + unit / blocks);
+    const uint32_t id = __ldg(&pairs[(tile + 1) * p.tile].x);
+    int64_t last = tile;  // the last tile that holds a piece
+    while (true) {
+      const int64_t other = last + 1 + lane;
+      const bool in_run = other < tiles && __ldg(&pairs[min(other, tiles - 1) * p.tile].x) == id;
+      const uint32_t votes = __ballot_sync(0xffffffffu, in_run);
+      last += __popc(votes);
+      if (votes != 0xffffffffu) break;
+    }
+    const int column = first_column<VECTOR, E>((int)(unit % blocks), lanes, lane);
+    const int count = lane < lanes ? owned_columns<VECTOR, E>(column, lanes, p.D) : 0;
+    if (count == 0) continue;
+    float sum[E], f[E];
+    Share<VECTOR, true, E> start;
+    start.load(p.pieces, (2 * tile + 1) * p.D + column, lanes, count);
+    start.unpack(ATTNRES_B200_FP32, sum);
+    for (int64_t next = tile + 1; next <= last; next += kJoinBatch) {
+      Share<VECTOR, true, E> raw[kJoinBatch];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      in_run[k] = next + k < tiles && __ldg(&pairs[(next + k) * p.tile].x) == id;
+      for (int k = 0; k < kJoinBatch; ++k)
+        if (next + k <= last) raw[k].load(p.pieces, 2 * (next + k) * p.D + column, lanes, count);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (in_run[k])
-        raw[k] = load_raw8<VECTOR>(p.pieces, ATTNRES_B200_FP32, 2 * (next + k) * p.D + column, lanes,
-                                   count);
+      for (int k = 0; k < kJoinBatch; ++k) {
+        if (next + k <= last) {
+          raw[k].unpack(ATTNRES_B200_FP32, f);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (in_run[k]) {
-        unpack_raw8(raw[k], ATTNRES_B200_FP32, f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] += f[e];
+          for (int e = 0; e < E; ++e) sum[e] += f[e];
+        }
       }
     }
-    if (!in_run[3]) break;
-    next += 4;
-  }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) sum[e] *= p.scale;
-  store8<VECTOR>(p.dtable, p.table_type, (int64_t)id * p.D + column, lanes, count, sum);
+    for (int e = 0; e < E; ++e) sum[e] *= p.scale;
+    store_share<VECTOR, E>(p.dtable, p.table_type, (int64_t)id * p.D + column, lanes, count, sum);
+  }
 }
 
 }  // namespace attnres_b200

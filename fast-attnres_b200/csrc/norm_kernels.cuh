@@ -8,8 +8,10 @@
 //
 // A row belongs to a group of WARPS warps that keeps it in registers, so it is read once and the
 // variance is the sum of squares of centred values (no cancellation, whatever the mean).  Groups
-// walk rows with a stride, hold the weights (and the sums of the parameter gradients) of their
-// columns in registers for the whole launch, and load rows ahead of the one they work on.
+// walk rows with a stride and hold the weights (and the sums of the parameter gradients) of their
+// columns in registers for the whole launch.  With 16-byte accesses a thread copies its own chunks
+// of the rows ahead into a shared-memory ring (cp.async: no barrier, each thread reads back only
+// what it copied itself), otherwise the next row waits in registers.
 #pragma once
 
 #include "typed_access.cuh"
@@ -32,55 +34,116 @@ struct NormParams {
   float* partials;   // backward: [gridDim.x, 2D], NULL when no parameter gradient is wanted
 };
 
-// Elements a thread owns: NJ chunks of CH consecutive ones (one 16-byte access each) with
-// VECTOR, otherwise NJ*CH single elements a group's width apart.
-template <typename T, bool VECTOR, int NJ, int WARPS>
+// What a thread owns of a row: E elements as pairs, in 16-byte chunks of CH consecutive ones with
+// VECTOR, otherwise single elements a group's width apart.
+template <typename T, bool VECTOR, int E, int WARPS>
 struct NormShape {
   static constexpr int kChunk = 16 / (int)sizeof(T);
-  static constexpr int kElements = NJ * kChunk;
+  static constexpr int kChunks = E / kChunk;
   static constexpr int kThreads = WARPS * 32;  // of a row group
-  static constexpr int kCapacity = kElements * kThreads;
+  static constexpr int kCapacity = E * kThreads;
 
   __device__ static int index(int k, int t) {
     return VECTOR ? ((k / kChunk) * kThreads + t) * kChunk + k % kChunk : k * kThreads + t;
   }
 
-  __device__ static void load(T* dst, const T* row, int D, int t) {
-    if constexpr (VECTOR) {
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int c = j * kThreads + t;
-        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        if (c * kChunk < D) raw = __ldg(reinterpret_cast<const uint4*>(row) + c);
-        *reinterpret_cast<uint4*>(dst + j * kChunk) = raw;
-      }
+  // The pairs of chunk j from its 16 bytes.
+  __device__ static void unpack(const uint4& raw, float2* f) {
+    if constexpr (sizeof(T) == 4) {
+      f[0] = make_float2(__uint_as_float(raw.x), __uint_as_float(raw.y));
+      f[1] = make_float2(__uint_as_float(raw.z), __uint_as_float(raw.w));
     } else {
+      const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-      for (int k = 0; k < kElements; ++k) {
-        const int i = k * kThreads + t;
-        dst[k] = i < D ? row[i] : T(0.f);
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (__is_same(T, __half)) f[k] = __half22float2(*reinterpret_cast<const __half2*>(&words[k]));
+        else f[k] = make_float2(bf16x2_lo(words[k]), bf16x2_hi(words[k]));
       }
     }
   }
 
-  __device__ static void store(T* row, const float* src, int D, int t) {
+  __device__ static void load(T* dst, const T* row, int D, int t) {
+    static_assert(!VECTOR, "rows of 16-byte chunks come through the ring");
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const int i = k * kThreads + t;
+      dst[k] = i < D ? row[i] : T(0.f);
+    }
+  }
+
+  __device__ static void store(T* row, const float2* src, int D, int t) {
+    const float* flat = reinterpret_cast<const float*>(src);
     if constexpr (VECTOR) {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
+      for (int j = 0; j < kChunks; ++j) {
         const int c = j * kThreads + t;
         if (c * kChunk < D) {
           __align__(16) T out[kChunk];
 #pragma unroll
-          for (int e = 0; e < kChunk; ++e) out[e] = from_float<T>(src[j * kChunk + e]);
+          for (int e = 0; e < kChunk; ++e) out[e] = from_float<T>(flat[j * kChunk + e]);
           *(reinterpret_cast<uint4*>(row) + c) = *reinterpret_cast<const uint4*>(out);
         }
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < kElements; ++k) {
+      for (int k = 0; k < E; ++k) {
         const int i = k * kThreads + t;
-        if (i < D) row[i] = from_float<T>(src[k]);
+        if (i < D) row[i] = from_float<T>(flat[k]);
       }
+    }
+  }
+
+  // [D] parameters of any type as this thread's pairs.
+  __device__ static void parameters(float2* dst, const void* base, int type, int D, int t,
+                                    float otherwise) {
+    if (base == nullptr) {
+#pragma unroll
+      for (int k = 0; k < E / 2; ++k) dst[k] = make_float2(otherwise, otherwise);
+      return;
+    }
+    if (VECTOR && (reinterpret_cast<uintptr_t>(base) & 15u) == 0) {  // chunk by chunk
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j) {
+        const int c = j * kThreads + t;
+        float f[8];
+        if (c * kChunk < D) {
+          if (type == ATTNRES_B200_FP32) {
+#pragma unroll
+            for (int k = 0; k < kChunk / 4; ++k) {
+              const float4 v = __ldg(static_cast<const float4*>(base) + c * (kChunk / 4) + k);
+              f[4 * k] = v.x;
+              f[4 * k + 1] = v.y;
+              f[4 * k + 2] = v.z;
+              f[4 * k + 3] = v.w;
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < kChunk / 4; ++k) {
+              const uint2 v = __ldg(static_cast<const uint2*>(base) + c * (kChunk / 4) + k);
+              const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
+              const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+              const bool bf16 = type == ATTNRES_B200_BF16;
+              f[4 * k] = bf16 ? bf16x2_lo(v.x) : lo.x;
+              f[4 * k + 1] = bf16 ? bf16x2_hi(v.x) : lo.y;
+              f[4 * k + 2] = bf16 ? bf16x2_lo(v.y) : hi.x;
+              f[4 * k + 3] = bf16 ? bf16x2_hi(v.y) : hi.y;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < kChunk; ++e) f[e] = otherwise;
+        }
+#pragma unroll
+        for (int k = 0; k < kChunk / 2; ++k)
+          dst[j * (kChunk / 2) + k] = make_float2(f[2 * k], f[2 * k + 1]);
+      }
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < E; k += 2) {
+      const int i = index(k, t), j = index(k + 1, t);
+      dst[k / 2].x = i < D ? load_typed(base, type, i) : otherwise;
+      dst[k / 2].y = j < D ? load_typed(base, type, j) : otherwise;
     }
   }
 };
@@ -111,123 +174,235 @@ __device__ __forceinline__ void group_sum(float* v, float* slots, int& parity, i
 
 constexpr int kNormThreads = 512;
 
-template <typename T, bool VECTOR, int NJ, int WARPS>
-__global__ void __launch_bounds__(kNormThreads)
-layer_norm_fwd_kernel(const NormParams p) {
-  using Shape = NormShape<T, VECTOR, NJ, WARPS>;
-  constexpr int E = Shape::kElements, TG = Shape::kThreads, GROUPS = kNormThreads / TG;
-  __shared__ float scratch[GROUPS][2 * WARPS];
-  const int group = threadIdx.x / TG, t = threadIdx.x % TG, D = p.D;
-  const float inv_width = 1.0f / (float)D;
-  float w[E], b[E];
+// Ring stages by what a CTA's rows take, and resident CTAs by what a thread holds in registers
+// (element-wise rows need registers for the next row as well).
+constexpr int norm_fwd_ctas(int E, bool vector) {
+  return vector ? (E <= 8 ? 3 : E <= 16 ? 2 : 1) : (E <= 8 ? 2 : 1);
+}
+constexpr int norm_grad_ctas(int E) { return E <= 8 ? 2 : 1; }
+
+template <typename Shape, int OPERANDS>
+struct NormRing {
+  static constexpr int kChunks = Shape::kChunks * OPERANDS;  // a thread's, a row
+  static constexpr int kStages = kChunks <= 1 ? 5 : kChunks <= 2 ? 4 : 3;
+  static constexpr uint32_t kBytes = (uint32_t)kStages * kChunks * kNormThreads * 16;
+
+  // Starts the copy of operand `which` of a row; chunks beyond D become zeros.
+  template <typename T>
+  __device__ static void copy(uint4* ring, int stage, int which, const T* row, int D, int t) {
 #pragma unroll
-  for (int k = 0; k < E; ++k) {
-    const int i = Shape::index(k, t);
-    w[k] = (p.weight != nullptr && i < D) ? load_typed(p.weight, p.param_type, i) : 1.f;
-    b[k] = (p.bias != nullptr && i < D) ? load_typed(p.bias, p.param_type, i) : 0.f;
+    for (int j = 0; j < Shape::kChunks; ++j) {
+      const int c = j * Shape::kThreads + t;
+      const bool inside = c * Shape::kChunk < D;
+      const uint4* src = reinterpret_cast<const uint4*>(row) + (inside ? c : 0);
+      const uint4* dst = at(ring, stage, which, j);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                       static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                   "l"(src), "r"(inside ? 16 : 0)
+                   : "memory");
+    }
   }
+  __device__ static uint4* at(uint4* ring, int stage, int which, int j) {
+    return ring + ((stage * kChunks + which * Shape::kChunks + j) * kNormThreads + threadIdx.x);
+  }
+  __device__ static void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  // The oldest of the rows in flight has arrived.
+  __device__ static void wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+  }
+  __device__ static void drain() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+  __device__ static void read(float2* dst, uint4* ring, int stage, int which) {
+#pragma unroll
+    for (int j = 0; j < Shape::kChunks; ++j)
+      Shape::unpack(*at(ring, stage, which, j), dst + j * (Shape::kChunk / 2));
+  }
+};
+
+extern __shared__ uint4 norm_smem[];
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+template <typename T, bool VECTOR, int E, int WARPS>
+__global__ void __launch_bounds__(kNormThreads, norm_fwd_ctas(E, VECTOR))
+layer_norm_fwd_kernel(const NormParams p) {
+  using Shape = NormShape<T, VECTOR, E, WARPS>;
+  using Ring = NormRing<Shape, 1>;
+  constexpr int TG = Shape::kThreads, GROUPS = kNormThreads / TG;
+  __shared__ float scratch[GROUPS][2 * WARPS];
+  // (the same number in every lane, and known to be: rows are addressed with uniform registers)
+  const int group = __shfl_sync(0xffffffffu, threadIdx.x / TG, 0), t = threadIdx.x % TG, D = p.D;
+  const float inv_width = 1.0f / (float)D;
   const T* x = static_cast<const T*>(p.x);
   const int64_t stride = (int64_t)gridDim.x * GROUPS;
   int64_t row = (int64_t)blockIdx.x * GROUPS + group;
-  __align__(16) T next[E];
-  if (row < p.N) Shape::load(next, x + row * p.x_row_stride, D, t);
+  T now[VECTOR ? 1 : E];
+  int stage = 0;
+  auto fetch = [&](int64_t which, int to) {
+    if constexpr (VECTOR) {
+      if (which < p.N) Ring::copy(norm_smem, to, 0, x + which * p.x_row_stride, D, t);
+      Ring::commit();
+    } else {
+      if (which < p.N) Shape::load(now, x + which * p.x_row_stride, D, t);
+    }
+  };
+  if constexpr (VECTOR) {
+#pragma unroll
+    for (int k = 0; k < Ring::kStages - 1; ++k) fetch(row + k * stride, k);
+  } else {
+    fetch(row, 0);
+  }
+  float2 w[E / 2], b[E / 2];
+  Shape::parameters(w, p.weight, p.param_type, D, t, 1.f);
+  Shape::parameters(b, p.bias, p.param_type, D, t, 0.f);
   int parity = 0;
   for (; row < p.N; row += stride) {
-    float f[E], sum[1] = {0.f};
+    float2 f[E / 2], part[2] = {both(0.f), both(0.f)};
+    if constexpr (VECTOR) {
+      // the stage that the previous row was read from
+      fetch(row + (Ring::kStages - 1) * stride, stage == 0 ? Ring::kStages - 1 : stage - 1);
+      Ring::wait();
+      Ring::read(f, norm_smem, stage, 0);
+      stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
+    } else {
 #pragma unroll
-    for (int k = 0; k < E; ++k) {
-      f[k] = to_float(next[k]);
-      sum[0] += f[k];
+      for (int k = 0; k < E / 2; ++k) f[k] = make_float2(to_float(now[2 * k]), to_float(now[2 * k + 1]));
+      fetch(row + stride, 0);
     }
-    if (row + stride < p.N) Shape::load(next, x + (row + stride) * p.x_row_stride, D, t);
+#pragma unroll
+    for (int k = 0; k < E / 2; ++k) part[k & 1] = __fadd2_rn(part[k & 1], f[k]);
+    float sum[1] = {(part[0].x + part[0].y) + (part[1].x + part[1].y)};
     group_sum<1, WARPS>(sum, scratch[group], parity, group, t);
     const float mean = sum[0] * inv_width;
-    sum[0] = 0.f;
 #pragma unroll
-    for (int k = 0; k < E; ++k) {
-      f[k] = Shape::index(k, t) < D ? f[k] - mean : 0.f;
-      sum[0] = fmaf(f[k], f[k], sum[0]);
+    for (int k = 0; k < E / 2; ++k) f[k] = __fadd2_rn(f[k], both(-mean));
+    if (D != Shape::kCapacity) {  // what lies beyond the row adds nothing to the variance
+#pragma unroll
+      for (int k = 0; k < E / 2; ++k) {
+        if (Shape::index(2 * k, t) >= D) f[k].x = 0.f;
+        if (Shape::index(2 * k + 1, t) >= D) f[k].y = 0.f;
+      }
     }
+    part[0] = part[1] = both(0.f);
+#pragma unroll
+    for (int k = 0; k < E / 2; ++k) part[k & 1] = __ffma2_rn(f[k], f[k], part[k & 1]);
+    sum[0] = (part[0].x + part[0].y) + (part[1].x + part[1].y);
     group_sum<1, WARPS>(sum, scratch[group], parity, group, t);
     const float rstd = rsqrtf(fmaf(sum[0], inv_width, p.eps));
 #pragma unroll
-    for (int k = 0; k < E; ++k) f[k] = fmaf(f[k] * rstd, w[k], b[k]);
+    for (int k = 0; k < E / 2; ++k) f[k] = __ffma2_rn(__fmul2_rn(f[k], both(rstd)), w[k], b[k]);
     Shape::store(static_cast<T*>(p.y) + row * D, f, D, t);
     if (t == 0 && p.stats != nullptr) {
       p.stats[row] = mean;
       p.stats[p.N + row] = rstd;
     }
   }
+  if constexpr (VECTOR) Ring::drain();
 }
 
-template <typename T, bool VECTOR, int NJ, int WARPS>
-__global__ void __launch_bounds__(kNormThreads)
+template <typename T, bool VECTOR, int E, int WARPS>
+__global__ void __launch_bounds__(kNormThreads, norm_grad_ctas(E))
 layer_norm_grad_kernel(const NormParams p) {
-  using Shape = NormShape<T, VECTOR, NJ, WARPS>;
-  constexpr int E = Shape::kElements, TG = Shape::kThreads, GROUPS = kNormThreads / TG;
+  using Shape = NormShape<T, VECTOR, E, WARPS>;
+  using Ring = NormRing<Shape, 2>;
+  constexpr int TG = Shape::kThreads, GROUPS = kNormThreads / TG;
   __shared__ float scratch[GROUPS][2 * 2 * WARPS];
-  extern __shared__ float group_rows[];  // [GROUPS - 1][2][capacity], used once at the end
-  const int group = threadIdx.x / TG, t = threadIdx.x % TG, D = p.D;
+  const int group = __shfl_sync(0xffffffffu, threadIdx.x / TG, 0), t = threadIdx.x % TG, D = p.D;
   const float inv_width = 1.0f / (float)D;
-  float w[E], dw[E], db[E];
-#pragma unroll
-  for (int k = 0; k < E; ++k) {
-    const int i = Shape::index(k, t);
-    w[k] = (p.weight != nullptr && i < D) ? load_typed(p.weight, p.param_type, i) : 1.f;
-    dw[k] = 0.f;
-    db[k] = 0.f;
-  }
   const T* x = static_cast<const T*>(p.x);
   const T* g = static_cast<const T*>(p.grad);
   const int64_t stride = (int64_t)gridDim.x * GROUPS;
   int64_t row = (int64_t)blockIdx.x * GROUPS + group;
-  __align__(16) T next_x[E];
-  __align__(16) T next_g[E];
+  T now_x[VECTOR ? 1 : E], now_g[VECTOR ? 1 : E];
   float next_mean = 0.f, next_rstd = 0.f;
-  if (row < p.N) {
-    Shape::load(next_x, x + row * p.x_row_stride, D, t);
-    Shape::load(next_g, g + row * p.grad_row_stride, D, t);
-    next_mean = p.stats[row];
-    next_rstd = p.stats[p.N + row];
+  int stage = 0;
+  auto fetch = [&](int64_t which, int to) {
+    if constexpr (VECTOR) {
+      if (which < p.N) {
+        Ring::copy(norm_smem, to, 0, x + which * p.x_row_stride, D, t);
+        Ring::copy(norm_smem, to, 1, g + which * p.grad_row_stride, D, t);
+      }
+      Ring::commit();
+    } else {
+      if (which < p.N) {
+        Shape::load(now_x, x + which * p.x_row_stride, D, t);
+        Shape::load(now_g, g + which * p.grad_row_stride, D, t);
+      }
+    }
+  };
+  auto fetch_stats = [&](int64_t which) {
+    if (which < p.N) {
+      next_mean = p.stats[which];
+      next_rstd = p.stats[p.N + which];
+    }
+  };
+  if constexpr (VECTOR) {
+#pragma unroll
+    for (int k = 0; k < Ring::kStages - 1; ++k) fetch(row + k * stride, k);
+  } else {
+    fetch(row, 0);
   }
+  fetch_stats(row);
+  float2 w[E / 2], dw[E / 2], db[E / 2];
+  Shape::parameters(w, p.weight, p.param_type, D, t, 1.f);
+#pragma unroll
+  for (int k = 0; k < E / 2; ++k) dw[k] = db[k] = both(0.f);
   int parity = 0;
   for (; row < p.N; row += stride) {
-    float xh[E], gw[E], sums[2] = {0.f, 0.f};
-    const float mean = next_mean, rstd = next_rstd;
+    float2 xh[E / 2], gw[E / 2];
+    if constexpr (VECTOR) {
+      fetch(row + (Ring::kStages - 1) * stride, stage == 0 ? Ring::kStages - 1 : stage - 1);
+      Ring::wait();
+      Ring::read(xh, norm_smem, stage, 0);
+      Ring::read(gw, norm_smem, stage, 1);
+      stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
+    } else {
 #pragma unroll
-    for (int k = 0; k < E; ++k) {
+      for (int k = 0; k < E / 2; ++k) {
+        xh[k] = make_float2(to_float(now_x[2 * k]), to_float(now_x[2 * k + 1]));
+        gw[k] = make_float2(to_float(now_g[2 * k]), to_float(now_g[2 * k + 1]));
+      }
+      fetch(row + stride, 0);
+    }
+    const float mean = next_mean, rstd = next_rstd;
+    fetch_stats(row + stride);
+    float2 sum_gw = both(0.f), sum_gwx = both(0.f);
+#pragma unroll
+    for (int k = 0; k < E / 2; ++k) {
       // Elements beyond D were loaded as zeros: their gradient is zero, so whatever xh they
       // get adds nothing to any sum.
-      xh[k] = (to_float(next_x[k]) - mean) * rstd;
-      const float gk = to_float(next_g[k]);
-      gw[k] = gk * w[k];
-      sums[0] += gw[k];
-      sums[1] = fmaf(gw[k], xh[k], sums[1]);
-      dw[k] = fmaf(gk, xh[k], dw[k]);
-      db[k] += gk;
-    }
-    if (row + stride < p.N) {
-      Shape::load(next_x, x + (row + stride) * p.x_row_stride, D, t);
-      Shape::load(next_g, g + (row + stride) * p.grad_row_stride, D, t);
-      next_mean = p.stats[row + stride];
-      next_rstd = p.stats[p.N + row + stride];
+      xh[k] = __fmul2_rn(__fadd2_rn(xh[k], both(-mean)), both(rstd));
+      dw[k] = __ffma2_rn(gw[k], xh[k], dw[k]);
+      db[k] = __fadd2_rn(db[k], gw[k]);
+      gw[k] = __fmul2_rn(gw[k], w[k]);
+      sum_gw = __fadd2_rn(sum_gw, gw[k]);
+      sum_gwx = __ffma2_rn(gw[k], xh[k], sum_gwx);
     }
     if (p.y != nullptr) {  // uniform over the grid
+      float sums[2] = {sum_gw.x + sum_gw.y, sum_gwx.x + sum_gwx.y};
       group_sum<2, WARPS>(sums, scratch[group], parity, group, t);
       const float mean_gw = sums[0] * inv_width, mean_gwx = sums[1] * inv_width;
 #pragma unroll
-      for (int k = 0; k < E; ++k) gw[k] = rstd * (gw[k] - mean_gw - xh[k] * mean_gwx);
+      for (int k = 0; k < E / 2; ++k) {
+        gw[k] = __ffma2_rn(xh[k], both(-mean_gwx), __fadd2_rn(gw[k], both(-mean_gw)));
+        gw[k] = __fmul2_rn(gw[k], both(rstd));
+      }
       Shape::store(static_cast<T*>(p.y) + row * D, gw, D, t);
     }
   }
+  if constexpr (VECTOR) Ring::drain();
   if (p.partials == nullptr) return;
-  // The groups' sums are added in index order, so the result does not depend on timing.
+  // The groups' sums are added in index order, so the result does not depend on timing.  They
+  // meet in the ring's memory, which nobody needs any more.
+  float* group_rows = reinterpret_cast<float*>(norm_smem);
+  float* sums_w = reinterpret_cast<float*>(dw);
+  float* sums_b = reinterpret_cast<float*>(db);
+  __syncthreads();
   if (group > 0) {
     float* mine = group_rows + (group - 1) * (2 * Shape::kCapacity);
 #pragma unroll
     for (int k = 0; k < E; ++k) {
-      mine[k * TG + t] = dw[k];
-      mine[Shape::kCapacity + k * TG + t] = db[k];
+      mine[k * TG + t] = sums_w[k];
+      mine[Shape::kCapacity + k * TG + t] = sums_b[k];
     }
   }
   __syncthreads();
@@ -237,13 +412,13 @@ layer_norm_grad_kernel(const NormParams p) {
   for (int k = 0; k < E; ++k) {
     for (int other = 0; other < GROUPS - 1; ++other) {
       const float* theirs = group_rows + other * (2 * Shape::kCapacity);
-      dw[k] += theirs[k * TG + t];
-      db[k] += theirs[Shape::kCapacity + k * TG + t];
+      sums_w[k] += theirs[k * TG + t];
+      sums_b[k] += theirs[Shape::kCapacity + k * TG + t];
     }
     const int i = Shape::index(k, t);
     if (i < D) {
-      out[i] = dw[k];
-      out[D + i] = db[k];
+      out[i] = sums_w[k];
+      out[D + i] = sums_b[k];
     }
   }
 }

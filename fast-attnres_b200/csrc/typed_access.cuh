@@ -41,74 +41,57 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Eight elements of one row as they lie in memory (the upper half is used by FP32 only), so that
-// loads can be issued ahead of the conversions.
-struct Raw8 {
-  uint4 a, b;
-};
+// A lane's share of one row as it lies in memory: eight consecutive elements (VECTOR: 16-byte
+// aligned and all valid), or E elements a step apart, so that neighbouring lanes read neighbouring
+// elements, of which the first `count` exist.  Whether elements are 4 or 2 bytes wide is a template
+// parameter (so that loads can be issued in batches, with no branch between them); which of the
+// two 16-bit types they are only matters to the conversion and is a runtime code.
+template <bool VECTOR, bool WIDE, int E = 8>
+struct Share {
+  static_assert(!VECTOR || E == 8, "a vector share is eight elements");
+  static constexpr int kWords = !VECTOR ? E : WIDE ? 8 : 4;
+  uint32_t w[kWords];
 
-// With VECTOR the eight are consecutive from `index`, 16-byte aligned and all valid.  Otherwise
-// element e is `index + e * step` (so that neighbouring lanes read neighbouring elements), and
-// only the first `count` exist.
-template <bool VECTOR>
-__device__ __forceinline__ Raw8 load_raw8(const void* base, int type, int64_t index, int step,
-                                          int count) {
-  Raw8 r;
-  r.a = make_uint4(0u, 0u, 0u, 0u);
-  r.b = r.a;
-  if constexpr (VECTOR) {
-    if (type == ATTNRES_B200_FP32) {
-      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(base) + index);
-      r.a = __ldg(p);
-      r.b = __ldg(p + 1);
-    } else {
-      r.a = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(base) + index));
-    }
-  } else {
-    uint32_t w[8];
-    if (type == ATTNRES_B200_FP32) {
+  __device__ __forceinline__ void load(const void* base, int64_t index, int step, int count) {
+    if constexpr (VECTOR) {
+      const char* p = static_cast<const char*>(base) + index * (WIDE ? 4 : 2);
+      *reinterpret_cast<uint4*>(w) = __ldg(reinterpret_cast<const uint4*>(p));
+      if constexpr (WIDE) *reinterpret_cast<uint4*>(w + 4) = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+    } else if constexpr (WIDE) {
       const uint32_t* p = static_cast<const uint32_t*>(base) + index;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = e < count ? __ldg(p + e * step) : 0u;
-      r.a = make_uint4(w[0], w[1], w[2], w[3]);
-      r.b = make_uint4(w[4], w[5], w[6], w[7]);
+      for (int e = 0; e < E; ++e) w[e] = e < count ? __ldg(p + e * step) : 0u;
     } else {
       const unsigned short* p = static_cast<const unsigned short*>(base) + index;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = e < count ? (uint32_t)__ldg(p + e * step) : 0u;
-      r.a = make_uint4(w[0] | (w[1] << 16), w[2] | (w[3] << 16), w[4] | (w[5] << 16),
-                       w[6] | (w[7] << 16));
+      for (int e = 0; e < E; ++e) w[e] = e < count ? (uint32_t)__ldg(p + e * step) : 0u;
     }
   }
-  return r;
-}
 
-__device__ __forceinline__ void unpack_raw8(const Raw8& r, int type, float* f) {
-  if (type == ATTNRES_B200_FP32) {
-    f[0] = __uint_as_float(r.a.x);
-    f[1] = __uint_as_float(r.a.y);
-    f[2] = __uint_as_float(r.a.z);
-    f[3] = __uint_as_float(r.a.w);
-    f[4] = __uint_as_float(r.b.x);
-    f[5] = __uint_as_float(r.b.y);
-    f[6] = __uint_as_float(r.b.z);
-    f[7] = __uint_as_float(r.b.w);
-  } else if (type == ATTNRES_B200_BF16) {
-    unpack8(r.a, f);
-  } else {
-    const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+  __device__ __forceinline__ void unpack(int type, float* f) const {
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-      f[2 * k] = v.x;
-      f[2 * k + 1] = v.y;
+      for (int e = 0; e < E; ++e) f[e] = __uint_as_float(w[e]);
+    } else if constexpr (VECTOR) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+        f[2 * k] = type == ATTNRES_B200_BF16 ? bf16x2_lo(w[k]) : h.x;
+        f[2 * k + 1] = type == ATTNRES_B200_BF16 ? bf16x2_hi(w[k]) : h.y;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        f[e] = type == ATTNRES_B200_BF16 ? bf16_bits_to_float(w[e])
+                                         : __half2float(__ushort_as_half((unsigned short)w[e]));
     }
   }
-}
+};
 
-template <bool VECTOR>
-__device__ __forceinline__ void store8(void* base, int type, int64_t index, int step, int count,
-                                       const float* f) {
+// Rounds and stores a share; `type` is the destination's.
+template <bool VECTOR, int E = 8>
+__device__ __forceinline__ void store_share(void* base, int type, int64_t index, int step, int count,
+                                            const float* f) {
   if constexpr (VECTOR) {
     if (type == ATTNRES_B200_FP32) {
       float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + index);
@@ -124,10 +107,21 @@ __device__ __forceinline__ void store8(void* base, int type, int64_t index, int 
       }
       *reinterpret_cast<uint4*>(static_cast<unsigned short*>(base) + index) = v;
     }
-  } else {
+  } else if (type == ATTNRES_B200_FP32) {
+    float* p = static_cast<float*>(base) + index;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < count) store_typed(base, type, index + e * step, f[e]);
+    for (int e = 0; e < E; ++e)
+      if (e < count) p[e * step] = f[e];
+  } else {
+    unsigned short w[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      w[e] = type == ATTNRES_B200_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f[e]))
+                                       : __half_as_ushort(__float2half_rn(f[e]));
+    unsigned short* p = static_cast<unsigned short*>(base) + index;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (e < count) p[e * step] = w[e];
   }
 }
 

@@ -119,6 +119,18 @@ def test_embed_many_tokens(n):
     _check(_ids((1, n), 5000, 7), _table(5000, 16, FP32), seed=8)
 
 
+@pytest.mark.parametrize("n,vocabulary,width,dtype,positions", [
+    (3000, 60000, 512, FP32, False), (3000, 60000, 513, BF16, True), (16384, 30000, 1024, FP32, True),
+    (1, 100000, 520, FP32, False), (40, 2000000, 24, FP32, False)])
+def test_embed_large_tables(n, vocabulary, width, dtype, positions):
+    """Tables whose zero rows take longer to write than the ids to sort: the first rows are written
+    beside the sort, the rest beside the sums; ids at both ends of both parts."""
+    tokens = _ids((1, n), vocabulary, 10)
+    if n > 3:
+        tokens[0, :3] = torch.tensor([0, vocabulary - 1, vocabulary // 3])
+    _check(tokens, _table(vocabulary, width, dtype), _table(n, width, dtype, 3) if positions else None)
+
+
 @pytest.mark.parametrize("padding_idx", [0, 5, -1])
 def test_embed_padding_row_gets_no_gradient(padding_idx):
     tokens = _ids((4, 90), 10)
