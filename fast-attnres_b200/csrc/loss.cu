@@ -29,8 +29,8 @@ constexpr int64_t kMaxLossRows = 1 << 30;
 constexpr int32_t kMaxLossVocabulary = 1 << 25;
 // Rows whose (max, sum) pairs are held at a time (65 536 x 250 pairs at 32 000 ids: 131 MB).
 constexpr int64_t kStatsRows = 65536;
-// Bytes of P held at a time.  A larger piece means fewer passes over the FP32 sums of dH; at
-// 16 384 rows two pieces cover 32 000 ids.
+// Bytes of P held at a time.  A larger piece means fewer FP32 slices of dH to add; at 16 384 rows
+// two pieces cover 32 000 ids.
 constexpr int64_t kPieceBytes = 512ll << 20;
 constexpr int64_t kPieceMinimum = 4096;
 
@@ -94,8 +94,17 @@ struct LossPlan {
   int64_t padded_weight;  // bytes of a padded copy of the weight
   int64_t stats_rows, partials;
   int64_t piece, pieces;  // ids of a piece
-  int64_t probs, running, weights;
+  int64_t slices;         // of dH, in each piece
+  int64_t probs, slices_out, weights;
 };
+
+int64_t tiles_of(int64_t rows, int64_t columns, bool pair) {
+  return ((rows + tile_rows(pair) - 1) / tile_rows(pair)) * ((columns + kTileN - 1) / kTileN);
+}
+
+// Pairs of CTAs load a third less for the same products; single CTAs make twice as many, smaller
+// tiles, which is what counts when there are few.
+bool use_pairs(int64_t tiles_of_pairs) { return tiles_of_pairs >= 148; }
 
 LossPlan plan_loss(int64_t N, int32_t V, int32_t D) {
   LossPlan plan;
@@ -110,32 +119,55 @@ LossPlan plan_loss(int64_t N, int32_t V, int32_t D) {
   plan.pieces = (V + plan.piece - 1) / plan.piece;
   const int64_t columns = plan.piece < V ? plan.piece : padded_width(V);
   plan.probs = align256(N * columns * 2);
-  plan.running = plan.pieces > 1 ? align256(N * D * (int64_t)sizeof(float)) : 0;
+  // dH has few tiles when there are few rows, each a long sum over the vocabulary: cut it so that
+  // there is one for every SM, but into sums of sixteen steps at least.
+  const int64_t tiles = tiles_of(N, D, false), steps = (plan.piece + kTileK - 1) / kTileK;
+  plan.slices = 148 / tiles;
+  if (plan.slices > steps / 16) plan.slices = steps / 16;
+  if (plan.slices < 1) plan.slices = 1;
+  const int64_t all = plan.slices * plan.pieces;
+  plan.slices_out = all > 1 ? align256(all * N * D * (int64_t)sizeof(float)) : 0;
   plan.weights = align256((N + 1) * (int64_t)sizeof(float));
   return plan;
 }
 
-template <int PASS, typename T>
-int launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& p_map,
-                   const ProductParams& p, int64_t tiles, int sms, cudaStream_t stream) {
+template <int PASS, typename T, bool PAIR>
+int launch_product(const CUtensorMap (&maps)[3], const ProductParams& p, int64_t tiles, int sms,
+                   cudaStream_t stream) {
   static SmemGrant grant;
-  if (int st = prepare_kernel(loss_product_kernel<PASS, T>, kProductSmem, grant)) return st;
-  const int grid = (int)(tiles < sms ? tiles : sms);
-  loss_product_kernel<PASS, T><<<grid, kProductThreads, kProductSmem, stream>>>(a, b, p_map, p);
-  return launched();
+  constexpr uint32_t smem = product_smem(PAIR);
+  if (int st = prepare_kernel(loss_product_kernel<PASS, T, PAIR>, smem, grant)) return st;
+  const int64_t workers = PAIR ? sms / 2 : sms;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)((tiles < workers ? tiles : workers) * (PAIR ? 2 : 1)));
+  config.blockDim = dim3(kProductThreads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = 2;
+  cluster.val.clusterDim.y = 1;
+  cluster.val.clusterDim.z = 1;
+  config.attrs = &cluster;
+  config.numAttrs = PAIR ? 1 : 0;
+  if (cudaLaunchKernelEx(&config, loss_product_kernel<PASS, T, PAIR>, maps[0], maps[1], maps[2],
+                         p) != cudaSuccess) {
+    cudaGetLastError();
+    return ATTNRES_B200_ERR_CUDA;
+  }
+  return ATTNRES_B200_OK;
 }
 
-template <int PASS>
-int launch_product_type(int32_t type, const CUtensorMap& a, const CUtensorMap& b,
-                        const CUtensorMap& p_map, const ProductParams& p, int64_t tiles, int sms,
-                        cudaStream_t stream) {
-  return type == ATTNRES_B200_BF16
-             ? launch_product<PASS, __nv_bfloat16>(a, b, p_map, p, tiles, sms, stream)
-             : launch_product<PASS, __half>(a, b, p_map, p, tiles, sms, stream);
-}
-
-int64_t tiles_of(int64_t rows, int64_t columns) {
-  return ((rows + kTileM - 1) / kTileM) * ((columns + kTileN - 1) / kTileN);
+// `tiles(pair)` counts the launch's tiles for pairs and for single CTAs.
+template <int PASS, typename Count>
+int launch_product_type(int32_t type, const CUtensorMap (&maps)[3], const ProductParams& p,
+                        Count tiles, int sms, cudaStream_t stream) {
+  const bool pair = use_pairs(tiles(true));
+  if (type == ATTNRES_B200_BF16)
+    return pair ? launch_product<PASS, __nv_bfloat16, true>(maps, p, tiles(true), sms, stream)
+                : launch_product<PASS, __nv_bfloat16, false>(maps, p, tiles(false), sms, stream);
+  return pair ? launch_product<PASS, __half, true>(maps, p, tiles(true), sms, stream)
+              : launch_product<PASS, __half, false>(maps, p, tiles(false), sms, stream);
 }
 
 // The weight as the TMA can read it: in place, or copied into rows of a multiple of eight.
@@ -160,7 +192,7 @@ extern "C" int64_t attnres_b200_loss_workspace_bytes(int64_t N, int32_t V, int32
   if (int st = check_loss(N, V, D, ATTNRES_B200_BF16, 1.f)) return -st;
   const LossPlan plan = plan_loss(N, V, D);
   if (!backward) return plan.padded_weight + plan.partials + align256(N * (int64_t)sizeof(float));
-  return plan.padded_weight + plan.probs + plan.running + plan.weights;
+  return plan.padded_weight + plan.probs + plan.slices_out + plan.weights;
 }
 
 extern "C" int attnres_b200_loss_forward(
@@ -216,9 +248,10 @@ extern "C" int attnres_b200_loss_forward(
   if (int st = launched()) return st;
   if (int st = lay_out_weight(&weight, &weight_row_stride, V, D, space, sms, cs)) return st;
 
-  CUtensorMap map_h, map_w;
-  if (int st = make_map(&map_h, kept, type, N, D, Dp, 64)) return st;
-  if (int st = make_map(&map_w, weight, type, V, D, V > 1 ? weight_row_stride : Dp, 64)) return st;
+  CUtensorMap maps[3];
+  if (int st = make_map(&maps[0], kept, type, N, D, Dp, 64)) return st;
+  if (int st = make_map(&maps[1], weight, type, V, D, V > 1 ? weight_row_stride : Dp, 64)) return st;
+  maps[2] = maps[1];  // nothing is stored through a map here
   ProductParams p{};
   p.count = count;
   p.N = (int32_t)N;
@@ -234,9 +267,8 @@ extern "C" int attnres_b200_loss_forward(
   for (int64_t row = 0; row < N; row += plan.stats_rows) {
     p.first_row = (int32_t)row;
     p.row_limit = (int32_t)(N - row < plan.stats_rows ? N - row : plan.stats_rows);
-    if (int st = launch_product_type<kStats>(type, map_h, map_w, map_w, p, tiles_of(p.row_limit, V),
-                                             sms, cs))
-      return st;
+    const auto tiles = [&](bool pair) { return tiles_of(p.row_limit, V, pair); };
+    if (int st = launch_product_type<kStats>(type, maps, p, tiles, sms, cs)) return st;
     loss_join_kernel<<<(p.row_limit + 7) / 8, 256, 0, cs>>>(partials, pairs, count, p.first_row,
                                                             p.row_limit, target_logit, kept_index,
                                                             lse2, losses);
@@ -273,9 +305,9 @@ extern "C" int attnres_b200_loss_backward(
   const int32_t Dp = padded_width(D);
   char* space = static_cast<char*>(workspace);
   void* probs = space + plan.padded_weight;
-  float* running = reinterpret_cast<float*>(space + plan.padded_weight + plan.probs);
+  float* slices_out = reinterpret_cast<float*>(space + plan.padded_weight + plan.probs);
   float* gradient_scale =
-      reinterpret_cast<float*>(space + plan.padded_weight + plan.probs + plan.running);
+      reinterpret_cast<float*>(space + plan.padded_weight + plan.probs + plan.slices_out);
   float* weight_of = gradient_scale + 1;
 
   if (int st = lay_out_weight(&weight, &weight_row_stride, V, D, space, sms, cs)) return st;
@@ -301,32 +333,38 @@ extern "C" int attnres_b200_loss_backward(
   p.lse2 = lse2;
   p.weight_of = weight_of;
   p.gradient_scale = gradient_scale;
-  p.running = running;
+  p.dhidden = dhidden;
+  p.dweight = dweight;
+  p.vector_dhidden = D % 8 == 0 && aligned16(dhidden);
+  p.vector_dweight = D % 8 == 0 && aligned16(dweight);
+  p.slices = (int32_t)plan.slices;
+  p.slices_out = plan.slices_out > 0 ? slices_out : nullptr;
   for (int64_t v0 = 0; v0 < V; v0 += plan.piece) {
     p.v0 = (int32_t)v0;
     p.vn = (int32_t)(V - v0 < plan.piece ? V - v0 : plan.piece);
-    p.first_piece = v0 == 0;
-    p.last_piece = v0 + p.vn == V;
-    CUtensorMap map_p, map_p_store;
     const int64_t stride = padded_width(p.vn);
-    if (int st = make_map(&map_p, probs, type, N, p.vn, stride, 64)) return st;
-    if (int st = make_map(&map_p_store, probs, type, N, p.vn, stride, 32)) return st;
-    if (int st = launch_product_type<kProbs>(type, map_h, map_w, map_p_store, p, tiles_of(N, p.vn),
-                                             sms, cs))
-      return st;
-    if (dhidden != nullptr) {
-      p.out = dhidden;
-      p.vector_out = D % 8 == 0 && aligned16(dhidden);
-      if (int st = launch_product_type<kHidden>(type, map_p, map_w, map_p, p, tiles_of(N, D), sms, cs))
-        return st;
-    }
-    if (dweight != nullptr) {
-      p.out = dweight;
-      p.vector_out = D % 8 == 0 && aligned16(dweight);
-      if (int st = launch_product_type<kWeight>(type, map_p, map_h, map_p, p, tiles_of(p.vn, D), sms,
-                                                cs))
-        return st;
-    }
+    CUtensorMap form[3] = {map_h, map_w, map_w}, use[3] = {map_h, map_w, map_h};
+    if (int st = make_map(&form[2], probs, type, N, p.vn, stride, 32)) return st;
+    if (int st = make_map(&use[0], probs, type, N, p.vn, stride, 64)) return st;
+    const auto logits = [&](bool pair) { return tiles_of(N, p.vn, pair); };
+    if (int st = launch_product_type<kProbs>(type, form, p, logits, sms, cs)) return st;
+    const auto gradients = [&](bool pair) {
+      return (dhidden ? tiles_of(N, D, pair) * plan.slices : 0) +
+             (dweight ? tiles_of(p.vn, D, pair) : 0);
+    };
+    if (int st = launch_product_type<kGradients>(type, use, p, gradients, sms, cs)) return st;
+    p.first_slice += p.slices;
   }
-  return ATTNRES_B200_OK;
+  if (dhidden == nullptr || p.slices_out == nullptr) return ATTNRES_B200_OK;
+  const int64_t ctas = (N + 7) / 8;
+  const unsigned grid = (unsigned)(ctas < 8 * sms ? ctas : 8 * sms);
+  if (type == ATTNRES_B200_BF16)
+    loss_slices_kernel<<<grid, 256, 0, cs>>>(slices_out, p.first_slice, count, kept_index,
+                                             gradient_scale, scale, N, D,
+                                             static_cast<__nv_bfloat16*>(dhidden), p.vector_dhidden);
+  else
+    loss_slices_kernel<<<grid, 256, 0, cs>>>(slices_out, p.first_slice, count, kept_index,
+                                             gradient_scale, scale, N, D,
+                                             static_cast<__half*>(dhidden), p.vector_dhidden);
+  return launched();
 }

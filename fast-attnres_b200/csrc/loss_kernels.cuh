@@ -5,11 +5,11 @@
 //   dH    = scale P W                    dW = scale P^T H
 //
 // Every product runs on the tensor cores with FP32 accumulators:
-//   kStats   tiles of z in tensor memory, reduced at once to a (max, sum) pair per row and half
-//            tile; a second kernel joins the pairs.  z never leaves the SM.
-//   kProbs   the same tiles again, turned into P (16-bit, the inputs' type) for one piece of the
-//            vocabulary;
-//   kHidden  dH from the piece, kWeight the piece's rows of dW.
+//   kStats      tiles of z in tensor memory, reduced at once to a (max, sum) pair per row and half
+//               tile; a second kernel joins the pairs.  z never leaves the SM.
+//   kProbs      the same tiles again, turned into P (16-bit, the inputs' type) for one piece of
+//               the vocabulary;
+//   kGradients  dH from the piece and the piece's rows of dW, in one launch.
 // Forming z twice costs a quarter of the training pass's products and saves [N, V] of memory.
 //
 // Rows whose target is the ignored id take no part: the kept rows are first gathered into
@@ -134,16 +134,25 @@ loss_pad_kernel(unsigned short* dst, const unsigned short* src, int64_t row_stri
 
 // ------------------------------------------------------------------------------ the products
 
-enum LossPass { kStats, kProbs, kHidden, kWeight };
+enum LossPass { kStats, kProbs, kGradients };
 
-constexpr int kTileM = 128, kTileN = 256, kTileK = 64;
+// A CTA alone forms tiles of 128 x 256; a pair of CTAs (PAIR) one of 256 x 256 with cta_group::2,
+// each holding 128 rows of A and of the result and half of B.  Alone, a CTA loads 48 KB for every
+// 128 x 256 x 64 products, which at the tensor cores' rate is more than the 64 bytes a cycle that
+// L2 gives an SM; in a pair it is 32 KB.
+constexpr int kTileN = 256, kTileK = 64;
 constexpr int kBoxBytes = 64 * 64 * 2;
-constexpr int kStageBytes = (kTileM + kTileN) / 64 * kBoxBytes;  // 48 KB
-constexpr int kStages = 4;
+constexpr int kCtaRows = 128;
+constexpr int tile_rows(bool pair) { return pair ? 256 : 128; }
+constexpr int stage_boxes_b(bool pair) { return pair ? 2 : 4; }
+constexpr int stage_bytes(bool pair) { return (2 + stage_boxes_b(pair)) * kBoxBytes; }
+constexpr int stage_count(bool pair) { return pair ? 6 : 4; }
 constexpr int kEpilogueWarps = 8;
 constexpr int kProductThreads = 64 + kEpilogueWarps * 32;
-constexpr int kStoreBytes = 32 * 64 * 2;  // a warp's 32 x 64 block of P
-constexpr uint32_t kProductSmem = kStages * kStageBytes + kEpilogueWarps * kStoreBytes + 1024;
+constexpr int kStoreBytes = 4096;  // a warp's block on its way out: 32 rows of 128 bytes
+constexpr uint32_t product_smem(bool pair) {
+  return stage_count(pair) * stage_bytes(pair) + kEpilogueWarps * kStoreBytes + 1024;
+}
 // FP16 keeps P times 2^15: probabilities of a large vocabulary would be subnormal.
 constexpr float kHalfLift = 32768.f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -162,11 +171,13 @@ struct ProductParams {
   float* target_logit;     // kStats: scale * log2(e) * z of the target
   const float* lse2;       // kProbs: log2 of the sum of exponentials
   const float* weight_of;  // kProbs: c_n over gradient_scale[0]
-  const float* gradient_scale;  // kHidden, kWeight
-  void* out;               // kHidden: [N, D]; kWeight: [V, D]
-  float* running;          // kHidden: FP32 [N, D] sums over the pieces (more than one piece)
-  int32_t first_piece, last_piece;
-  int32_t vector_out;      // rows of `out` allow 16-byte stores
+  const float* gradient_scale;  // kGradients
+  void* dhidden;           // kGradients: [N, D] or NULL
+  void* dweight;           // kGradients: [V, D] or NULL
+  float* slices_out;       // dH in several slices of the vocabulary: FP32 [slices][N, D]
+  int32_t first_slice;     // of this piece
+  int32_t slices;          // that this piece is cut into
+  int32_t vector_dhidden, vector_dweight;  // their rows allow 16-byte stores
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -186,56 +197,162 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return pack_half2(lo, hi);
 }
 
-// Tiles in the order in which CTAs take them.  z: sixteen row tiles share each column tile while
-// it is in L2.  Gradients: the few column tiles of a row tile run side by side, so P is read once.
-template <int PASS>
-__device__ __forceinline__ void tile_at(int index, int tiles_m, int tiles_n, int* m, int* n) {
-  if constexpr (PASS == kStats || PASS == kProbs) {
-    constexpr int kGroup = 16;
-    const int group = index / (kGroup * tiles_n), rest = index - group * kGroup * tiles_n;
-    const int height = min(kGroup, tiles_m - group * kGroup);
-    *n = rest / height;
-    *m = group * kGroup + rest - *n * height;
-  } else {
-    *m = index / tiles_n;
-    *n = index - *m * tiles_n;
-  }
+__device__ __forceinline__ void store_shared16(uint32_t smem, uint32_t a, uint32_t b, uint32_t c,
+                                               uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+__device__ __forceinline__ uint4 load_shared16(uint32_t smem) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(smem)
+               : "memory");
+  return v;
 }
 
-// Warp 0 loads, warp 1 multiplies, warps 2..9 take finished tiles out of tensor memory while the
-// next one is formed in its other half.
-template <int PASS, typename T>
+// A warp's block waits in shared memory as 32 rows of 128 bytes, 16-byte chunk c of row r at
+// c ^ (r mod 8): the TMA's 128-byte swizzle, and free of bank conflicts both ways.
+__device__ __forceinline__ uint32_t block_slot(uint32_t staging, int row, int chunk) {
+  return staging + row * 128 + ((chunk ^ (row & 7)) << 4);
+}
+
+// Writes the block out row by row, so that a store covers whole lines: `mine` is the element offset
+// in `out` of this lane's row, or negative when that row has no place; `columns` (of 128 bytes'
+// worth) are valid.
+template <typename T>
+__device__ __forceinline__ void write_block(uint32_t staging, T* out, int64_t mine, int columns,
+                                            bool vector, int lane) {
+  constexpr int per_chunk = 16 / (int)sizeof(T), width = 8 * per_chunk;
+  __syncwarp();
+  if (vector) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = i * 4 + (lane >> 3), chunk = lane & 7;
+      const int64_t offset = __shfl_sync(0xffffffffu, mine, row);
+      if (offset >= 0 && chunk * per_chunk < columns)
+        *reinterpret_cast<uint4*>(out + offset + chunk * per_chunk) =
+            load_shared16(block_slot(staging, row, chunk));
+    }
+  } else {
+    for (int row = 0; row < 32; ++row) {
+      const int64_t offset = __shfl_sync(0xffffffffu, mine, row);
+      if (offset < 0) continue;
+#pragma unroll
+      for (int c = 0; c < width; c += 32) {
+        const int column = c + lane;
+        const uint32_t slot =
+            block_slot(staging, row, column / per_chunk) + column % per_chunk * (int)sizeof(T);
+        if (column < columns) {
+          if constexpr (sizeof(T) == 4) {
+            float v;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(slot) : "memory");
+            out[offset + column] = v;
+          } else {
+            unsigned short v;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(slot) : "memory");
+            reinterpret_cast<unsigned short*>(out)[offset + column] = v;
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+}
+
+// One tile's place in its product: which matrices, where it begins, which steps along K.
+struct Tile {
+  int m, n;           // first row and column of the result
+  int k_first, k_steps;
+  bool weight;        // kGradients: dW rather than dH
+  int slice;          // of dH
+};
+
+// The tiles of a launch in the order in which CTAs take them.  z: 2048 rows share each column tile
+// while it is in L2.  Gradients: the few column tiles of a row tile run side by side, so P comes
+// from memory once; dH first, its sums are the longer ones when there are few rows.
+template <int PASS, bool PAIR>
+struct TileOrder {
+  static constexpr int kRows = tile_rows(PAIR);
+  int tiles_m, tiles_n, steps;     // kGradients: of dH
+  int weight_m, weight_steps, slice_steps;
+  int hidden_tiles, total;
+
+  __device__ TileOrder(const ProductParams& p, int kept) {
+    if constexpr (PASS == kGradients) {
+      tiles_n = (p.D + kTileN - 1) / kTileN;
+      tiles_m = p.dhidden != nullptr ? (kept + kRows - 1) / kRows : 0;
+      steps = (p.vn + kTileK - 1) / kTileK;
+      slice_steps = (steps + p.slices - 1) / p.slices;
+      weight_m = p.dweight != nullptr ? (p.vn + kRows - 1) / kRows : 0;
+      weight_steps = (kept + kTileK - 1) / kTileK;
+      hidden_tiles = tiles_m * tiles_n * p.slices;
+      total = hidden_tiles + weight_m * tiles_n;
+    } else {
+      const int rows = PASS == kStats ? min(max(kept - p.first_row, 0), p.row_limit) : kept;
+      tiles_m = (rows + kRows - 1) / kRows;
+      tiles_n = (p.vn + kTileN - 1) / kTileN;
+      steps = (p.D + kTileK - 1) / kTileK;
+      total = tiles_m * tiles_n;
+    }
+  }
+
+  __device__ Tile at(int index) const {
+    Tile t;
+    t.weight = false;
+    t.slice = 0;
+    t.k_first = 0;
+    if constexpr (PASS == kGradients) {
+      t.weight = index >= hidden_tiles;
+      int rest = index;
+      if (t.weight) {
+        rest -= hidden_tiles;
+        t.k_steps = weight_steps;
+      } else {
+        const int per_slice = tiles_m * tiles_n;
+        t.slice = index / per_slice;
+        rest = index - t.slice * per_slice;
+        t.k_first = t.slice * slice_steps;
+        t.k_steps = max(0, min(slice_steps, steps - t.k_first));
+      }
+      const int row = rest / tiles_n;
+      t.m = row * kRows;
+      t.n = (rest - row * tiles_n) * kTileN;
+    } else {
+      constexpr int kGroup = 2048 / kRows;
+      const int group = index / (kGroup * tiles_n), rest = index - group * kGroup * tiles_n;
+      const int height = min(kGroup, tiles_m - group * kGroup);
+      const int column = rest / height;
+      t.m = (group * kGroup + rest - column * height) * kRows;
+      t.n = column * kTileN;
+      t.k_steps = steps;
+    }
+    return t;
+  }
+};
+
+// Warp 0 loads, warp 1 multiplies (in a pair: the first CTA's, for both), warps 2..9 take finished
+// tiles out of tensor memory while the next one is formed in its other half.
+// Maps: kStats, kProbs: kept rows, head, P (to store).  kGradients: P, head, kept rows.
+template <int PASS, typename T, bool PAIR>
 __global__ void __launch_bounds__(kProductThreads, 1)
-loss_product_kernel(const __grid_constant__ CUtensorMap map_a,
-                    const __grid_constant__ CUtensorMap map_b,
-                    const __grid_constant__ CUtensorMap map_p, const ProductParams p) {
-  constexpr bool kAmn = PASS == kWeight, kBmn = PASS == kHidden || PASS == kWeight;
-  constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
-  constexpr uint32_t kInstruction = mma_instruction(kBf16, kAmn, kBmn, kTileM, kTileN);
-  extern __shared__ unsigned char product_smem[];
+loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
+                    const __grid_constant__ CUtensorMap map_1,
+                    const __grid_constant__ CUtensorMap map_2, const ProductParams p) {
+  constexpr bool kBf16 = !__is_same(T, __half);
+  constexpr int kRows = tile_rows(PAIR), kStages = stage_count(PAIR);
+  constexpr int kStageBytes = stage_bytes(PAIR), kBoxesB = stage_boxes_b(PAIR);
+  extern __shared__ unsigned char product_memory[];
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages], done[2], taken[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t stages = (smem_addr(product_smem) + 1023u) & ~1023u;
-
+  const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;
+  const int worker = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
+  const int workers = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
+  const uint32_t stages = (smem_addr(product_memory) + 1023u) & ~1023u;
   const int kept = *p.count;
-  int tiles_m, tiles_n, k_steps;
-  if constexpr (PASS == kStats || PASS == kProbs) {
-    const int rows = PASS == kStats ? min(max(kept - p.first_row, 0), p.row_limit) : kept;
-    tiles_m = (rows + kTileM - 1) / kTileM;
-    tiles_n = (p.vn + kTileN - 1) / kTileN;
-    k_steps = (p.D + kTileK - 1) / kTileK;
-  } else if constexpr (PASS == kHidden) {
-    tiles_m = (kept + kTileM - 1) / kTileM;
-    tiles_n = (p.D + kTileN - 1) / kTileN;
-    k_steps = (p.vn + kTileK - 1) / kTileK;
-  } else {
-    tiles_m = (p.vn + kTileM - 1) / kTileM;
-    tiles_n = (p.D + kTileN - 1) / kTileN;
-    k_steps = (kept + kTileK - 1) / kTileK;
-  }
-  const int tiles = tiles_m * tiles_n;
+  const TileOrder<PASS, PAIR> order(p, kept);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -244,17 +361,18 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a,
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&done[b], 1);
-      mbar_init(&taken[b], kEpilogueWarps);
+      mbar_init(&taken[b], kEpilogueWarps * (PAIR ? 2 : 1));
     }
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    prefetch_tensor_map(&map_a);
-    prefetch_tensor_map(&map_b);
+    prefetch_tensor_map(&map_0);
+    prefetch_tensor_map(&map_1);
   }
-  if (warp == 1) tmem_alloc_512(&tmem_slot);
+  if (warp == 1) tmem_alloc_512<PAIR>(&tmem_slot);
   __syncwarp();
   tcgen05_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_barrier();  // the other CTA's barriers exist
   tcgen05_fence_after();
   const uint32_t tmem = tmem_slot;
 
@@ -263,30 +381,32 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a,
       int stage = 0;
       uint32_t phase = 0;
       bool alive = true;
-      for (int i = blockIdx.x; i < tiles && alive; i += gridDim.x) {
-        int m, n;
-        tile_at<PASS>(i, tiles_m, tiles_n, &m, &n);
-        // Where the operands' rows (K-major) or columns (MN-major) of this tile begin.
-        const int a0 = PASS == kStats ? p.first_row + m * kTileM : m * kTileM;
-        const int b0 = (PASS == kStats || PASS == kProbs) ? p.v0 + n * kTileN : n * kTileN;
-        const int bk = PASS == kHidden ? p.v0 : 0;
-        for (int k = 0; k < k_steps; ++k) {
+      for (int i = worker; i < order.total && alive; i += workers) {
+        const Tile t = order.at(i);
+        // Where this CTA's operands begin along M and N, and which tensors they come from.
+        const bool a_mn = PASS == kGradients && t.weight;
+        const CUtensorMap* map_b = PASS == kGradients && t.weight ? &map_2 : &map_1;
+        const int a0 = t.m + rank * kCtaRows + (PASS == kStats ? p.first_row : 0);
+        const int b0 = t.n + rank * (kTileN / 2) + (PASS == kGradients ? 0 : p.v0);
+        const int bk = PASS == kGradients && !t.weight ? p.v0 : 0;
+        for (int k = t.k_first; k < t.k_first + t.k_steps; ++k) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, &abort_flag)) {
             alive = false;
             break;
           }
-          mbar_expect_tx(&full[stage], kStageBytes);
-          const uint32_t a = stages + stage * kStageBytes, b = a + kTileM / 64 * kBoxBytes;
+          uint32_t bar = smem_addr(&full[stage]);
+          if constexpr (PAIR) bar = cluster_address(bar, 0);
+          if (rank == 0) mbar_expect_tx(&full[stage], kStageBytes * (PAIR ? 2 : 1));
+          const uint32_t a = stages + stage * kStageBytes, b = a + 2 * kBoxBytes;
 #pragma unroll
-          for (int j = 0; j < kTileM / 64; ++j) {
-            if constexpr (kAmn) tensor_load_2d(a + j * kBoxBytes, &map_a, a0 + j * 64, k * kTileK, &full[stage]);
-            else tensor_load_2d(a + j * kBoxBytes, &map_a, k * kTileK, a0 + j * 64, &full[stage]);
-          }
+          for (int j = 0; j < 2; ++j)
+            tensor_load_2d<PAIR>(a + j * kBoxBytes, &map_0, a_mn ? a0 + j * 64 : k * kTileK,
+                                 a_mn ? k * kTileK : a0 + j * 64, bar);
 #pragma unroll
-          for (int j = 0; j < kTileN / 64; ++j) {
-            if constexpr (kBmn) tensor_load_2d(b + j * kBoxBytes, &map_b, b0 + j * 64, bk + k * kTileK, &full[stage]);
-            else tensor_load_2d(b + j * kBoxBytes, &map_b, k * kTileK, b0 + j * 64, &full[stage]);
-          }
+          for (int j = 0; j < kBoxesB; ++j)
+            tensor_load_2d<PAIR>(b + j * kBoxBytes, map_b,
+                                 PASS == kGradients ? b0 + j * 64 : k * kTileK,
+                                 PASS == kGradients ? bk + k * kTileK : b0 + j * 64, bar);
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
@@ -295,35 +415,42 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a,
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       int stage = 0, buffer = 0;
       uint32_t phase = 0, buffer_phase = 0;
       bool alive = true;
-      for (int i = blockIdx.x; i < tiles && alive; i += gridDim.x) {
+      for (int i = worker; i < order.total && alive; i += workers) {
+        const Tile t = order.at(i);
         if (!mbar_wait(&taken[buffer], buffer_phase ^ 1u, &abort_flag)) break;
         tcgen05_fence_after();
         const uint32_t d = tmem + buffer * kTileN;
-        for (int k = 0; k < k_steps; ++k) {
+        // 16 elements of K: 32 bytes along a K-major row, two 1 KB groups of MN-major rows.
+        const bool a_mn = PASS == kGradients && t.weight;
+        const uint32_t instruction = a_mn
+            ? mma_instruction(kBf16, true, PASS == kGradients, kRows, kTileN)
+            : mma_instruction(kBf16, false, PASS == kGradients, kRows, kTileN);
+        const uint32_t step_a = (a_mn ? 2048 : 32) >> 4;
+        constexpr uint32_t step_b = (PASS == kGradients ? 2048 : 32) >> 4;
+        for (int k = 0; k < t.k_steps; ++k) {
           if (!mbar_wait(&full[stage], phase, &abort_flag)) {
             alive = false;
             break;
           }
           tcgen05_fence_after();
-          const uint32_t a = stages + stage * kStageBytes, b = a + kTileM / 64 * kBoxBytes;
-          // 16 elements of K: 32 bytes along a K-major row, two 1 KB groups of MN-major rows.
+          const uint32_t a = stages + stage * kStageBytes, b = a + 2 * kBoxBytes;
           const uint64_t da = operand_descriptor(a), db = operand_descriptor(b);
 #pragma unroll
           for (int kk = 0; kk < kTileK / 16; ++kk)
-            tcgen05_mma_f16(d, da + kk * (kAmn ? 2048 >> 4 : 32 >> 4),
-                            db + kk * (kBmn ? 2048 >> 4 : 32 >> 4), kInstruction, k > 0 || kk > 0);
-          tcgen05_commit(&empty[stage]);
+            tcgen05_mma_f16<PAIR>(d, da + kk * step_a, db + kk * step_b, instruction,
+                                  k > 0 || kk > 0);
+          tcgen05_commit<PAIR>(&empty[stage]);
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
         if (!alive) break;
-        tcgen05_commit(&done[buffer]);
+        tcgen05_commit<PAIR>(&done[buffer]);
         buffer ^= 1;
         if (buffer == 0) buffer_phase ^= 1u;
       }
@@ -333,15 +460,19 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a,
     const uint32_t staging = stages + kStages * kStageBytes + (warp - 2) * kStoreBytes;
     const float to_log2 = p.scale * kLog2e;
     float out_scale = 0.f;
-    if constexpr (PASS == kHidden || PASS == kWeight)
+    if constexpr (PASS == kGradients)
       out_scale = p.scale * *p.gradient_scale * (kBf16 ? 1.f : 1.f / kHalfLift);
+    uint32_t taken_bar[2] = {smem_addr(&taken[0]), smem_addr(&taken[1])};
+    if constexpr (PAIR) {
+      taken_bar[0] = cluster_address(taken_bar[0], 0);
+      taken_bar[1] = cluster_address(taken_bar[1], 0);
+    }
     int buffer = 0;
     uint32_t buffer_phase = 0;
-    for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
-      int m, n;
-      tile_at<PASS>(i, tiles_m, tiles_n, &m, &n);
-      const int row = m * kTileM + quad * 32 + lane;  // of the tile's matrix
-      const int column = n * kTileN + half * (kTileN / 2);
+    for (int i = worker; i < order.total; i += workers) {
+      const Tile t = order.at(i);
+      const int first_row = t.m + rank * kCtaRows + quad * 32, row = first_row + lane;
+      const int column = t.n + half * (kTileN / 2);
       // What the row needs is fetched while the products run.
       int target = -1;
       float lse2 = 0.f, weight_of = 0.f;
@@ -389,9 +520,11 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a,
           sum = fmaf(sum, exp2_approx(top - pivot), part);
           top = high;
         }
-        if (live) p.partials[(int64_t)row * (2 * tiles_n) + 2 * n + half] = make_float2(top, sum);
+        if (live)
+          p.partials[(int64_t)row * (2 * order.tiles_n) + 2 * (t.n / kTileN) + half] =
+              make_float2(top, sum);
       } else if constexpr (PASS == kProbs) {
-        const bool rows_exist = m * kTileM + quad * 32 < p.N;
+        const bool rows_exist = first_row < p.N;
 #pragma unroll 1
         for (int c = 0; c < kTileN / 2 && column + c < p.vn; c += 64) {
           if (lane == 0) tensor_store_wait_read();
@@ -412,69 +545,69 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a,
               for (int e = 0; e < 32; ++e) v[e] = 0.f;
             }
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const uint32_t w0 = pack2<T>(v[8 * q], v[8 * q + 1]);
-              const uint32_t w1 = pack2<T>(v[8 * q + 2], v[8 * q + 3]);
-              const uint32_t w2 = pack2<T>(v[8 * q + 4], v[8 * q + 5]);
-              const uint32_t w3 = pack2<T>(v[8 * q + 6], v[8 * q + 7]);
-              const uint32_t slot = staging + lane * 128 + (((h * 4 + q) ^ (lane & 7)) << 4);
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot), "r"(w0), "r"(w1),
-                           "r"(w2), "r"(w3)
-                           : "memory");
-            }
+            for (int q = 0; q < 4; ++q)
+              store_shared16(block_slot(staging, lane, h * 4 + q), pack2<T>(v[8 * q], v[8 * q + 1]),
+                             pack2<T>(v[8 * q + 2], v[8 * q + 3]),
+                             pack2<T>(v[8 * q + 4], v[8 * q + 5]),
+                             pack2<T>(v[8 * q + 6], v[8 * q + 7]));
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0 && rows_exist)
-            tensor_store_2d(&map_p, column + c, m * kTileM + quad * 32, staging);
+          if (lane == 0 && rows_exist) tensor_store_2d(&map_2, column + c, first_row, staging);
         }
-      } else {
-        const int rows = PASS == kHidden ? kept : p.vn;
-        int64_t out_row = 0;
-        if (row < rows) out_row = PASS == kHidden ? p.kept_index[row] : p.v0 + row;
-        T* out = static_cast<T*>(p.out) + out_row * p.D;
-        float* running = PASS == kHidden ? p.running + (int64_t)row * p.D : nullptr;
+      } else if (!t.weight && p.slices_out != nullptr) {
+        // A slice of dH: FP32, added to the others by loss_slices_kernel.
+        const int64_t place = ((int64_t)(p.first_slice + t.slice) * p.N + row) * p.D + column;
 #pragma unroll 1
         for (int c = 0; c < kTileN / 2 && column + c < p.D; c += 32) {
           uint32_t r[32];
           tmem_load_32(src + c, r);
-          float v[32];
-          const int base = column + c, valid = min(32, p.D - base);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = k_steps > 0 ? __uint_as_float(r[e]) : 0.f;
-          if (row < rows) {
-            if (PASS == kHidden && !p.first_piece) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (e < valid) v[e] += running[base + e];
-            }
-            if (PASS == kHidden && !p.last_piece) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (e < valid) running[base + e] = v[e];
-            } else if (p.vector_out) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                if (8 * q < valid) {
-                  uint4 w;
-                  w.x = pack2<T>(v[8 * q] * out_scale, v[8 * q + 1] * out_scale);
-                  w.y = pack2<T>(v[8 * q + 2] * out_scale, v[8 * q + 3] * out_scale);
-                  w.z = pack2<T>(v[8 * q + 4] * out_scale, v[8 * q + 5] * out_scale);
-                  w.w = pack2<T>(v[8 * q + 6] * out_scale, v[8 * q + 7] * out_scale);
-                  *reinterpret_cast<uint4*>(out + base + 8 * q) = w;
-                }
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (e < valid) out[base + e] = from_float<T>(v[e] * out_scale);
-            }
+          for (int q = 0; q < 8; ++q) {
+            if (t.k_steps > 0)
+              store_shared16(block_slot(staging, lane, q), r[4 * q], r[4 * q + 1], r[4 * q + 2],
+                             r[4 * q + 3]);
+            else
+              store_shared16(block_slot(staging, lane, q), 0u, 0u, 0u, 0u);
           }
+          write_block<float>(staging, p.slices_out + c, row < kept ? place : -1, p.D - column - c,
+                             p.D % 4 == 0, lane);
+        }
+      } else {
+        int64_t place = -1;
+        if (t.weight) {
+          if (row < p.vn) place = (int64_t)(p.v0 + row) * p.D + column;
+        } else if (row < kept) {
+          place = (int64_t)p.kept_index[row] * p.D + column;
+        }
+        T* out = static_cast<T*>(t.weight ? p.dweight : p.dhidden);
+        const bool vector = t.weight ? p.vector_dweight : p.vector_dhidden;
+#pragma unroll 1
+        for (int c = 0; c < kTileN / 2 && column + c < p.D; c += 64) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t r[32];
+            tmem_load_32(src + c + h * 32, r);
+            float v[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              v[e] = t.k_steps > 0 ? __uint_as_float(r[e]) * out_scale : 0.f;  // no kept row: zeros
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              store_shared16(block_slot(staging, lane, h * 4 + q), pack2<T>(v[8 * q], v[8 * q + 1]),
+                             pack2<T>(v[8 * q + 2], v[8 * q + 3]),
+                             pack2<T>(v[8 * q + 4], v[8 * q + 5]),
+                             pack2<T>(v[8 * q + 6], v[8 * q + 7]));
+          }
+          write_block<T>(staging, out + c, place, p.D - column - c, vector, lane);
         }
       }
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&taken[buffer]);
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_cluster(taken_bar[buffer]);
+        else mbar_arrive(&taken[buffer]);
+      }
       buffer ^= 1;
       if (buffer == 0) buffer_phase ^= 1u;
     }
@@ -483,14 +616,65 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a,
   __syncwarp();
   tcgen05_fence_before();
   __syncthreads();
-  tcgen05_fence_after();
   if (abort_flag != 0) {  // copies and products still in flight land before anything is given back
     const uint64_t start = global_timer_ns();
     while (global_timer_ns() - start < 200000ull) {
     }
     __syncthreads();
   }
-  if (warp == 1) tmem_dealloc_512(tmem);
+  // Nobody leaves while the other CTA may still read its memory or signal its barriers.
+  if constexpr (PAIR) cluster_barrier();
+  tcgen05_fence_after();
+  if (warp == 1) tmem_dealloc_512<PAIR>(tmem);
+  if constexpr (PAIR) cluster_barrier();
+}
+
+// dH from its slices, added in order; one warp a kept row.
+template <typename T>
+__global__ void __launch_bounds__(256)
+loss_slices_kernel(const float* __restrict__ slices, int count, const int32_t* kept_rows,
+                   const int32_t* __restrict__ kept_index, const float* gradient_scale, float scale,
+                   int64_t N, int D, T* out, int vector) {
+  const float out_scale = scale * *gradient_scale * (__is_same(T, __half) ? 1.f / kHalfLift : 1.f);
+  const int lane = threadIdx.x & 31, kept = *kept_rows;
+  const int64_t all = N * D;
+  for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < kept;
+       row += (int64_t)gridDim.x * 8) {
+    const float* mine = slices + row * D;
+    T* to = out + (int64_t)kept_index[row] * D;
+    if (vector) {
+#pragma unroll 2
+      for (int c = lane * 8; c < D; c += 256) {
+        float sum[8] = {};
+#pragma unroll 4
+        for (int s = 0; s < count; ++s) {
+          const float4* from = reinterpret_cast<const float4*>(mine + s * all + c);
+          const float4 a = __ldcs(from), b = __ldcs(from + 1);
+          sum[0] += a.x;
+          sum[1] += a.y;
+          sum[2] += a.z;
+          sum[3] += a.w;
+          sum[4] += b.x;
+          sum[5] += b.y;
+          sum[6] += b.z;
+          sum[7] += b.w;
+        }
+        uint4 v;
+        v.x = pack2<T>(sum[0] * out_scale, sum[1] * out_scale);
+        v.y = pack2<T>(sum[2] * out_scale, sum[3] * out_scale);
+        v.z = pack2<T>(sum[4] * out_scale, sum[5] * out_scale);
+        v.w = pack2<T>(sum[6] * out_scale, sum[7] * out_scale);
+        *reinterpret_cast<uint4*>(to + c) = v;
+      }
+    } else {
+      for (int c = lane; c < D; c += 32) {
+        float sum = 0.f;
+#pragma unroll 4
+        for (int s = 0; s < count; ++s) sum += __ldcs(mine + s * all + c);
+        to[c] = from_float<T>(sum * out_scale);
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------ joining the loss

@@ -112,6 +112,19 @@ def test_linear_cross_entropy_matches_the_definition(rows, vocabulary, width, dt
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("rows,vocabulary,width", [
+    (2500, 6001, 136),      # pairs of CTAs for the logits, single ones for the gradients
+    (3001, 20003, 264),     # pairs for both
+    (200, 30000, 40),       # dH in slices of the vocabulary
+    (2900, 20003, 517)])    # pairs, element-wise rows
+def test_linear_cross_entropy_every_kind_of_product(rows, vocabulary, width, dtype):
+    hidden, weight, targets = _case(rows, vocabulary, width, dtype, ignored=0.1, seed=14)
+    first = _check(hidden, weight, targets)
+    second = _check(hidden, weight, targets)
+    assert all(torch.equal(a, b) for a, b in zip(first, second)), "not the same bits twice"
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 @pytest.mark.parametrize("ignored", [0.0, 0.5, 0.98])
 @pytest.mark.parametrize("scale", [1.0, -0.5])
