@@ -82,7 +82,9 @@ SIGNATURES = {
     "attnres_b200_loss_forward": (c_int32, [
         c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_int32, c_int32,
         c_int32, c_int64, c_float, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-        c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "attnres_b200_loss_gradients_in_forward": (c_int32, [c_int32, c_int32, c_int32]),
+    "attnres_b200_loss_scale_gradient": (c_int32, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "attnres_b200_loss_backward": (c_int32, [
         c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_int32, c_int32,
         c_int32, c_int64, c_float, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -280,13 +282,24 @@ def embedding_backward(*arguments) -> None:
     check(load().attnres_b200_embedding_backward(*arguments), "attnres_b200_embedding_backward")
 
 
-def loss_workspace_bytes(N, V, D, backward_pass) -> int:
-    return _sized(load().attnres_b200_loss_workspace_bytes(N, V, D, int(backward_pass)),
+LOSS_FORWARD, LOSS_BACKWARD, LOSS_FORWARD_GRADIENTS = 0, 1, 2
+
+
+def loss_workspace_bytes(N, V, D, which) -> int:
+    return _sized(load().attnres_b200_loss_workspace_bytes(N, V, D, int(which)),
                   "attnres_b200_loss_workspace_bytes")
 
 
 def loss_forward(*arguments) -> None:
     check(load().attnres_b200_loss_forward(*arguments), "attnres_b200_loss_forward")
+
+
+def loss_gradients_in_forward(D, type_code, reduction) -> bool:
+    return bool(load().attnres_b200_loss_gradients_in_forward(D, type_code, reduction))
+
+
+def loss_scale_gradient(*arguments) -> None:
+    check(load().attnres_b200_loss_scale_gradient(*arguments), "attnres_b200_loss_scale_gradient")
 
 
 def loss_backward(*arguments) -> None:

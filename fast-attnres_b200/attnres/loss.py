@@ -17,8 +17,9 @@ import torch
 from . import _calls, _native
 from ._sources import MAX_WIDTH, _first_failure, check_scalar
 
-# Compiled operators (csrc/torch_ops.cpp): `linear_cross_entropy_forward` and `..._backward` launch
-# the kernels, `linear_cross_entropy` is the differentiable call over the two.
+# Compiled operators (csrc/torch_ops.cpp): `linear_cross_entropy_forward` and `..._backward`, or
+# `..._with_gradients` and `..._scale_gradient`, launch the kernels; `linear_cross_entropy` is the
+# differentiable call over either pair.
 _ops = _native.load_operators()
 _linear_cross_entropy = _ops.linear_cross_entropy.default
 _TYPES = _calls.HALVES
@@ -46,6 +47,18 @@ def _(grad, weight, targets, kept, index, count, sums, ignored, reduction, scale
       need_weight):
     return (weight.new_empty((*targets.shape, weight.shape[1]) if need_hidden else (0,)),
             weight.new_empty(weight.shape if need_weight else (0,)))
+
+
+@torch.library.register_fake("attnres_b200::linear_cross_entropy_with_gradients")
+def _(hidden, weight, targets, ignored, reduction, scale, need_hidden, need_weight):
+    return (_loss_like(hidden, targets, reduction),
+            hidden.new_empty(hidden.shape if need_hidden else (0,)),
+            hidden.new_empty(weight.shape if need_weight else (0,)))
+
+
+@torch.library.register_fake("attnres_b200::linear_cross_entropy_scale_gradient")
+def _(gradient, upstream):
+    return torch.empty_like(gradient, memory_format=torch.contiguous_format)
 
 
 @torch.library.register_fake("attnres_b200::linear_cross_entropy")
@@ -108,6 +121,11 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     ``targets``).  The loss is FP32; products run on the tensor cores with FP32 accumulators, and
     the softmax residue is rounded to the inputs' type before it is multiplied into the gradients,
     which come back in that type.  Differentiable once; results are the same bits every time.
+
+    A BF16 mean or sum over rows of 512 features and more forms its gradients in the forward, from
+    the same logits (so evaluate under ``torch.no_grad()``); the backward multiplies them by the
+    upstream gradient, one more rounding unless that is a power of two.  Every other call forms the
+    logits a second time in the backward.
     """
     if not (_acceptable(hidden, weight, targets) and type(ignore_index) is int
             and reduction in _REDUCTIONS and _calls.plain_number(scale) and math.isfinite(scale)):

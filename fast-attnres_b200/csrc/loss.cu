@@ -29,9 +29,9 @@ constexpr int64_t kMaxLossRows = 1 << 30;
 constexpr int32_t kMaxLossVocabulary = 1 << 25;
 // Rows whose (max, sum) pairs are held at a time (65 536 x 250 pairs at 32 000 ids: 131 MB).
 constexpr int64_t kStatsRows = 65536;
-// Bytes of P held at a time.  A larger piece means fewer FP32 slices of dH to add; at 16 384 rows
-// two pieces cover 32 000 ids.
-constexpr int64_t kPieceBytes = 512ll << 20;
+// Bytes of P held at a time.  More pieces mean more FP32 parts of a gradient to add; 16 384 rows of
+// 32 000 ids are one piece.
+constexpr int64_t kPieceBytes = 1024ll << 20;
 constexpr int64_t kPieceMinimum = 4096;
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -131,6 +131,28 @@ LossPlan plan_loss(int64_t N, int32_t V, int32_t D) {
   return plan;
 }
 
+// The forward that forms the gradients as well works on pieces of the rows.
+struct GradientPlan {
+  int64_t piece, pieces;  // rows
+  int64_t partials, codes, weight_parts;
+};
+
+GradientPlan plan_gradients(int64_t N, int32_t V, int32_t D) {
+  GradientPlan plan;
+  int64_t most = kPieceBytes / (2 * (int64_t)padded_width(V)) / 256 * 256;
+  if (most < 1024) most = 1024;
+  plan.pieces = (N + most - 1) / most;
+  plan.piece = ((N + plan.pieces - 1) / plan.pieces + 255) / 256 * 256;
+  if (plan.piece > N) plan.piece = N;
+  plan.pieces = (N + plan.piece - 1) / plan.piece;
+  const int64_t tiles_n = (V + kTileN - 1) / kTileN;
+  plan.partials = align256(plan.piece * 2 * tiles_n * (int64_t)sizeof(float2));
+  plan.codes = align256(plan.piece * (int64_t)padded_width(V) * 2);
+  plan.weight_parts =
+      plan.pieces > 1 ? align256(plan.pieces * V * (int64_t)D * (int64_t)sizeof(float)) : 0;
+  return plan;
+}
+
 template <int PASS, typename T, bool PAIR>
 int launch_product(const CUtensorMap (&maps)[3], const ProductParams& p, int64_t tiles, int sms,
                    cudaStream_t stream) {
@@ -188,10 +210,17 @@ int lay_out_weight(const void** weight, int64_t* row_stride, int32_t V, int32_t 
 using namespace attnres_b200;
 
 extern "C" int64_t attnres_b200_loss_workspace_bytes(int64_t N, int32_t V, int32_t D,
-                                                     int32_t backward) {
+                                                     int32_t pass) {
   if (int st = check_loss(N, V, D, ATTNRES_B200_BF16, 1.f)) return -st;
   const LossPlan plan = plan_loss(N, V, D);
-  if (!backward) return plan.padded_weight + plan.partials + align256(N * (int64_t)sizeof(float));
+  const int64_t logits = align256(N * (int64_t)sizeof(float));
+  if (pass == ATTNRES_B200_LOSS_FORWARD) return plan.padded_weight + plan.partials + logits;
+  if (pass == ATTNRES_B200_LOSS_FORWARD_GRADIENTS) {
+    const GradientPlan gradients = plan_gradients(N, V, D);
+    return plan.padded_weight + gradients.partials + logits + 256 + gradients.codes +
+           gradients.weight_parts;
+  }
+  if (pass != ATTNRES_B200_LOSS_BACKWARD) return -ATTNRES_B200_ERR_BAD_FLAGS;
   return plan.padded_weight + plan.probs + plan.slices_out + plan.weights;
 }
 
@@ -199,18 +228,24 @@ extern "C" int attnres_b200_loss_forward(
     const void* hidden, int64_t hidden_row_stride, const void* weight, int64_t weight_row_stride,
     const void* targets, int32_t targets_64, int64_t N, int32_t V, int32_t D, int32_t type,
     int64_t ignored, float scale, int32_t reduction, void* kept, int32_t* kept_index,
-    int32_t* kept_target, int32_t* count, float* lse2, float* losses, float* loss, void* workspace,
-    int64_t workspace_bytes, void* stream) {
+    int32_t* kept_target, int32_t* count, float* lse2, float* losses, float* loss, void* dhidden,
+    void* dweight, void* workspace, int64_t workspace_bytes, void* stream) {
   if (int st = check_loss(N, V, D, type, scale)) return st;
+  const bool gradients = dhidden != nullptr || dweight != nullptr;
+  if (gradients && type != ATTNRES_B200_BF16) return ATTNRES_B200_ERR_BAD_TYPE;
+  if (gradients && reduction == ATTNRES_B200_LOSS_NONE) return ATTNRES_B200_ERR_BAD_FLAGS;
   if (reduction < ATTNRES_B200_LOSS_NONE || reduction > ATTNRES_B200_LOSS_MEAN)
     return ATTNRES_B200_ERR_BAD_FLAGS;
-  if (!hidden || !weight || !targets || !kept || !kept_index || !kept_target || !count || !lse2 ||
-      !losses || !workspace || (reduction != ATTNRES_B200_LOSS_NONE && !loss))
+  if (!hidden || !weight || !targets || !kept || !kept_index || !kept_target || !count ||
+      (!gradients && !lse2) || !losses || !workspace ||
+      (reduction != ATTNRES_B200_LOSS_NONE && !loss))
     return ATTNRES_B200_ERR_NULL_POINTER;
   if (!aligned2(hidden) || !aligned2(weight) || !aligned16(kept) || !aligned16(workspace) ||
+      !aligned2(dhidden) || !aligned2(dweight) ||
       (reinterpret_cast<uintptr_t>(targets) & (targets_64 ? 7u : 3u)) != 0)
     return ATTNRES_B200_ERR_MISALIGNED;
-  if (workspace_bytes < attnres_b200_loss_workspace_bytes(N, V, D, 0))
+  const int32_t pass = gradients ? ATTNRES_B200_LOSS_FORWARD_GRADIENTS : ATTNRES_B200_LOSS_FORWARD;
+  if (workspace_bytes < attnres_b200_loss_workspace_bytes(N, V, D, pass))
     return ATTNRES_B200_ERR_WORKSPACE;
   int device = 0, sms = 0;
   if (int st = current_device(&device)) return st;
@@ -219,8 +254,14 @@ extern "C" int attnres_b200_loss_forward(
   const LossPlan plan = plan_loss(N, V, D);
   const int32_t Dp = padded_width(D);
   char* space = static_cast<char*>(workspace);
+  const GradientPlan pieces = plan_gradients(N, V, D);
   float2* partials = reinterpret_cast<float2*>(space + plan.padded_weight);
-  float* target_logit = reinterpret_cast<float*>(space + plan.padded_weight + plan.partials);
+  char* rest = space + plan.padded_weight + (gradients ? pieces.partials : plan.partials);
+  float* target_logit = reinterpret_cast<float*>(rest);
+  rest += align256(N * (int64_t)sizeof(float));
+  float* gradient_scale = reinterpret_cast<float*>(rest);  // from here on with gradients only
+  unsigned short* codes = reinterpret_cast<unsigned short*>(rest + 256);
+  float* weight_parts = reinterpret_cast<float*>(rest + 256 + pieces.codes);
 
   GatherParams g{};
   g.hidden = hidden;
@@ -240,6 +281,11 @@ extern "C" int attnres_b200_loss_forward(
   g.count = count;
   g.target_logit = target_logit;
   g.losses = losses;
+  if (gradients) {
+    g.gradient_scale = gradient_scale;
+    g.mean = reduction == ATTNRES_B200_LOSS_MEAN;
+    g.dhidden = static_cast<unsigned short*>(dhidden);
+  }
   const int gather_grid = (int)((N + g.block_rows - 1) / g.block_rows);
   if (D % 8 == 0 && aligned16(hidden) && (N == 1 || hidden_row_stride % 8 == 0))
     loss_gather_kernel<true><<<gather_grid, kGatherThreads, 0, cs>>>(g);
@@ -264,14 +310,48 @@ extern "C" int attnres_b200_loss_forward(
   p.partials = partials;
   p.target_logit = target_logit;
   const int pairs = 2 * ((V + kTileN - 1) / kTileN);
-  for (int64_t row = 0; row < N; row += plan.stats_rows) {
+  if (gradients) {
+    const int64_t stride = padded_width(V);
+    p.kept_index = kept_index;
+    p.gradient_scale = gradient_scale;
+    p.dhidden = dhidden;
+    p.dweight = dweight;
+    p.vector_dhidden = D % 8 == 0 && aligned16(dhidden);
+    p.vector_dweight = D % 8 == 0 && aligned16(dweight);
+    p.slices = 1;
+    for (int64_t piece = 0; piece < pieces.pieces; ++piece) {
+      p.first_row = (int32_t)(piece * pieces.piece);
+      p.row_limit = (int32_t)(N - p.first_row < pieces.piece ? N - p.first_row : pieces.piece);
+      CUtensorMap form[3] = {maps[0], maps[1], maps[1]}, use[3] = {maps[0], maps[1], maps[0]};
+      if (int st = make_map(&form[2], codes, type, p.row_limit, V, stride, 32)) return st;
+      if (int st = make_map(&use[0], codes, type, p.row_limit, V, stride, 64)) return st;
+      const auto logits = [&](bool pair) { return tiles_of(p.row_limit, V, pair); };
+      if (int st = launch_product_type<kCodes>(type, form, p, logits, sms, cs)) return st;
+      loss_probs_kernel<<<p.row_limit < 8 * sms ? p.row_limit : 8 * sms, kJoinThreads, 0, cs>>>(
+          partials, pairs, count, p.first_row, p.row_limit, target_logit, kept_target, kept_index,
+          losses, codes, stride, V);
+      if (int st = launched()) return st;
+      p.weight_out = dweight != nullptr && pieces.pieces > 1 ? weight_parts + piece * V * D : nullptr;
+      const auto both = [&](bool pair) {
+        return (dhidden ? tiles_of(p.row_limit, D, pair) : 0) + (dweight ? tiles_of(V, D, pair) : 0);
+      };
+      if (int st = launch_product_type<kGradients>(type, use, p, both, sms, cs)) return st;
+    }
+    if (p.weight_out != nullptr) {
+      loss_slices_kernel<<<8 * sms, 256, 0, cs>>>(weight_parts, (int)pieces.pieces, nullptr, nullptr,
+                                                  gradient_scale, scale, V, D,
+                                                  static_cast<__nv_bfloat16*>(dweight),
+                                                  p.vector_dweight);
+      if (int st = launched()) return st;
+    }
+  }
+  for (int64_t row = 0; row < N && !gradients; row += plan.stats_rows) {
     p.first_row = (int32_t)row;
     p.row_limit = (int32_t)(N - row < plan.stats_rows ? N - row : plan.stats_rows);
     const auto tiles = [&](bool pair) { return tiles_of(p.row_limit, V, pair); };
     if (int st = launch_product_type<kStats>(type, maps, p, tiles, sms, cs)) return st;
-    loss_join_kernel<<<(p.row_limit + 7) / 8, 256, 0, cs>>>(partials, pairs, count, p.first_row,
-                                                            p.row_limit, target_logit, kept_index,
-                                                            lse2, losses);
+    loss_join_kernel<<<p.row_limit < 8 * sms ? p.row_limit : 8 * sms, kJoinThreads, 0, cs>>>(
+        partials, pairs, count, p.first_row, p.row_limit, target_logit, kept_index, lse2, losses);
     if (int st = launched()) return st;
   }
   if (reduction == ATTNRES_B200_LOSS_NONE) return ATTNRES_B200_OK;
@@ -295,7 +375,7 @@ extern "C" int attnres_b200_loss_backward(
   if (!aligned2(weight) || !aligned16(kept) || !aligned16(workspace) || !aligned2(dhidden) ||
       !aligned2(dweight) || (reinterpret_cast<uintptr_t>(targets) & (targets_64 ? 7u : 3u)) != 0)
     return ATTNRES_B200_ERR_MISALIGNED;
-  if (workspace_bytes < attnres_b200_loss_workspace_bytes(N, V, D, 1))
+  if (workspace_bytes < attnres_b200_loss_workspace_bytes(N, V, D, ATTNRES_B200_LOSS_BACKWARD))
     return ATTNRES_B200_ERR_WORKSPACE;
   int device = 0, sms = 0;
   if (int st = current_device(&device)) return st;
@@ -332,6 +412,7 @@ extern "C" int attnres_b200_loss_backward(
   p.kept_target = kept_target;
   p.lse2 = lse2;
   p.weight_of = weight_of;
+  p.row_limit = (int32_t)N;
   p.gradient_scale = gradient_scale;
   p.dhidden = dhidden;
   p.dweight = dweight;
@@ -366,5 +447,28 @@ extern "C" int attnres_b200_loss_backward(
     loss_slices_kernel<<<grid, 256, 0, cs>>>(slices_out, p.first_slice, count, kept_index,
                                              gradient_scale, scale, N, D,
                                              static_cast<__half*>(dhidden), p.vector_dhidden);
+  return launched();
+}
+
+extern "C" int32_t attnres_b200_loss_gradients_in_forward(int32_t D, int32_t type, int32_t reduction) {
+  // The gradients' own forward saves the second z (2 N V D products) and spends 4 N V bytes on
+  // turning codes into P, which ties near D = 450 at 1.4 PFLOP/s and 6.5 TB/s.  FP16 stays with the
+  // backward: its gradients before the upstream factor may be too small for the type.
+  return type == ATTNRES_B200_BF16 && reduction != ATTNRES_B200_LOSS_NONE && D >= 512;
+}
+
+extern "C" int attnres_b200_loss_scale_gradient(const void* gradient, const float* upstream,
+                                                int64_t elements, void* out, void* stream) {
+  if (elements < 1) return ATTNRES_B200_ERR_BAD_ROWS;
+  if (!gradient || !upstream || !out) return ATTNRES_B200_ERR_NULL_POINTER;
+  if (!aligned16(gradient) || !aligned16(out)) return ATTNRES_B200_ERR_MISALIGNED;
+  int device = 0, sms = 0;
+  if (int st = current_device(&device)) return st;
+  if (int st = sm_count(device, &sms)) return st;
+  const int64_t ctas = (elements / 8 + 1023) / 1024 + 1;
+  loss_scale_kernel<<<(unsigned)(ctas < 16 * sms ? ctas : 16 * sms), 256, 0,
+                      static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const __nv_bfloat16*>(gradient), upstream, elements,
+      static_cast<__nv_bfloat16*>(out));
   return launched();
 }

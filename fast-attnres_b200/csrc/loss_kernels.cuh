@@ -10,7 +10,13 @@
 //   kProbs      the same tiles again, turned into P (16-bit, the inputs' type) for one piece of
 //               the vocabulary;
 //   kGradients  dH from the piece and the piece's rows of dW, in one launch.
-// Forming z twice costs a quarter of the training pass's products and saves [N, V] of memory.
+// The backward forms z a second time: that costs a quarter of the training pass's products and no
+// memory.  Where the loss is one number, its gradients are known up to that number's upstream
+// gradient, and the forward can form them at once, from one z (kCodes instead of kStats):
+//   kCodes      a piece of the rows: (max, sum) pairs as above, and z as 16-bit codes, the distance
+//               from the half tile's maximum in steps of 2^-11 powers of two (a probability is off
+//               by 2^-12.5 at most, an eighth of what P's own rounding to BF16 allows);
+//   loss_probs_kernel joins a row's pairs and turns its codes into P in place.
 //
 // Rows whose target is the ignored id take no part: the kept rows are first gathered into
 // consecutive ones (their number stays on the device), so padding costs no products and whatever
@@ -40,6 +46,11 @@ struct GatherParams {
   int32_t* count;
   float* target_logit;      // [N], to be filled in by the products
   float* losses;            // [N]: zero for ignored rows
+  // The gradients' common scale for an upstream gradient of one, and dH, whose ignored rows are
+  // zeroed; NULL where the forward forms no gradients.
+  float* gradient_scale;
+  int32_t mean;
+  unsigned short* dhidden;
 };
 
 __device__ __forceinline__ int64_t load_target(const void* targets, int wide, int64_t n) {
@@ -112,12 +123,18 @@ __global__ void __launch_bounds__(kGatherThreads) loss_gather_kernel(const Gathe
                          static_cast<const unsigned short*>(p.hidden) +
                              (base + r) * p.hidden_row_stride,
                          p.D, p.Dp, lane);
+      else if (p.dhidden != nullptr)
+        for (int i = lane; i < p.D; i += 32) p.dhidden[(base + r) * p.D + i] = 0;
     }
     place += total;
     __syncthreads();
   }
   if (last == p.N) {  // the last CTA knows how many there are
-    if (tid == 0) *p.count = place;
+    if (tid == 0) {
+      *p.count = place;
+      if (p.gradient_scale != nullptr)  // no kept row: the gradients are zeros
+        *p.gradient_scale = place == 0 ? 0.f : p.mean ? 1.f / (float)place : 1.f;
+    }
     const int64_t padded = min(p.N, ((int64_t)place + 127) / 128 * 128);
     for (int64_t r = place + warp; r < padded; r += kGatherThreads / 32)
       copy_row<VECTOR>(p.kept + r * p.Dp, nullptr, p.D, p.Dp, lane);
@@ -134,7 +151,7 @@ loss_pad_kernel(unsigned short* dst, const unsigned short* src, int64_t row_stri
 
 // ------------------------------------------------------------------------------ the products
 
-enum LossPass { kStats, kProbs, kGradients };
+enum LossPass { kStats, kProbs, kGradients, kCodes };
 
 // A CTA alone forms tiles of 128 x 256; a pair of CTAs (PAIR) one of 256 x 256 with cta_group::2,
 // each holding 128 rows of A and of the result and half of B.  Alone, a CTA loads 48 KB for every
@@ -155,20 +172,21 @@ constexpr uint32_t product_smem(bool pair) {
 }
 // FP16 keeps P times 2^15: probabilities of a large vocabulary would be subnormal.
 constexpr float kHalfLift = 32768.f;
+constexpr float kCodeSteps = 2048.f;  // of a code, to a power of two
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct ProductParams {
   const int32_t* count;  // kept rows
   int32_t N, V, D;
-  int32_t first_row;     // kStats: rows [first_row, first_row + row_limit)
+  int32_t first_row;     // kept rows [first_row, first_row + row_limit)
   int32_t row_limit;
   int32_t v0, vn;        // the piece: ids [v0, v0 + vn)
   float scale;
   const int32_t* kept_index;
   const int32_t* kept_target;
-  float2* partials;        // kStats: [row_limit][2 tiles_n] (max, sum) in powers of two
-  float* target_logit;     // kStats: scale * log2(e) * z of the target
+  float2* partials;        // kStats, kCodes: [row_limit][2 tiles_n] (max, sum) in powers of two
+  float* target_logit;     // kStats, kCodes: scale * log2(e) * z of the target
   const float* lse2;       // kProbs: log2 of the sum of exponentials
   const float* weight_of;  // kProbs: c_n over gradient_scale[0]
   const float* gradient_scale;  // kGradients
@@ -177,6 +195,7 @@ struct ProductParams {
   float* slices_out;       // dH in several slices of the vocabulary: FP32 [slices][N, D]
   int32_t first_slice;     // of this piece
   int32_t slices;          // that this piece is cut into
+  float* weight_out;       // dW from several pieces of the rows: FP32 [V, D] of this piece
   int32_t vector_dhidden, vector_dweight;  // their rows allow 16-byte stores
 };
 
@@ -278,18 +297,17 @@ struct TileOrder {
   int weight_m, weight_steps, slice_steps;
   int hidden_tiles, total;
 
-  __device__ TileOrder(const ProductParams& p, int kept) {
+  __device__ TileOrder(const ProductParams& p, int rows) {
     if constexpr (PASS == kGradients) {
       tiles_n = (p.D + kTileN - 1) / kTileN;
-      tiles_m = p.dhidden != nullptr ? (kept + kRows - 1) / kRows : 0;
+      tiles_m = p.dhidden != nullptr ? (rows + kRows - 1) / kRows : 0;
       steps = (p.vn + kTileK - 1) / kTileK;
       slice_steps = (steps + p.slices - 1) / p.slices;
       weight_m = p.dweight != nullptr ? (p.vn + kRows - 1) / kRows : 0;
-      weight_steps = (kept + kTileK - 1) / kTileK;
+      weight_steps = (rows + kTileK - 1) / kTileK;
       hidden_tiles = tiles_m * tiles_n * p.slices;
       total = hidden_tiles + weight_m * tiles_n;
     } else {
-      const int rows = PASS == kStats ? min(max(kept - p.first_row, 0), p.row_limit) : kept;
       tiles_m = (rows + kRows - 1) / kRows;
       tiles_n = (p.vn + kTileN - 1) / kTileN;
       steps = (p.D + kTileK - 1) / kTileK;
@@ -333,7 +351,7 @@ struct TileOrder {
 
 // Warp 0 loads, warp 1 multiplies (in a pair: the first CTA's, for both), warps 2..9 take finished
 // tiles out of tensor memory while the next one is formed in its other half.
-// Maps: kStats, kProbs: kept rows, head, P (to store).  kGradients: P, head, kept rows.
+// Maps: kGradients: P, head, kept rows; the others: kept rows, head, P or codes (to store).
 template <int PASS, typename T, bool PAIR>
 __global__ void __launch_bounds__(kProductThreads, 1)
 loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
@@ -351,7 +369,8 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
   const int worker = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
   const int workers = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
   const uint32_t stages = (smem_addr(product_memory) + 1023u) & ~1023u;
-  const int kept = *p.count;
+  // Kept rows of this launch, counted from first_row on.
+  const int kept = min(max(*p.count - p.first_row, 0), p.row_limit);
   const TileOrder<PASS, PAIR> order(p, kept);
 
   if (threadIdx.x == 0) {
@@ -386,9 +405,9 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
         // Where this CTA's operands begin along M and N, and which tensors they come from.
         const bool a_mn = PASS == kGradients && t.weight;
         const CUtensorMap* map_b = PASS == kGradients && t.weight ? &map_2 : &map_1;
-        const int a0 = t.m + rank * kCtaRows + (PASS == kStats ? p.first_row : 0);
+        const int a0 = t.m + rank * kCtaRows + (PASS != kGradients ? p.first_row : 0);
         const int b0 = t.n + rank * (kTileN / 2) + (PASS == kGradients ? 0 : p.v0);
-        const int bk = PASS == kGradients && !t.weight ? p.v0 : 0;
+        const int bk = PASS != kGradients ? 0 : t.weight ? p.first_row : p.v0;
         for (int k = t.k_first; k < t.k_first + t.k_steps; ++k) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, &abort_flag)) {
             alive = false;
@@ -477,48 +496,78 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
       int target = -1;
       float lse2 = 0.f, weight_of = 0.f;
       bool live = true;
-      if constexpr (PASS == kStats) {
-        live = p.first_row + row < kept && row < p.row_limit;
-        if (live) target = p.kept_target[p.first_row + row];
-      } else if constexpr (PASS == kProbs) {
+      if constexpr (PASS != kGradients) {
         live = row < kept;
+        if (live) target = p.kept_target[p.first_row + row];
+      }
+      if constexpr (PASS == kProbs) {
+        target = target >= p.v0 ? target - p.v0 : -1;
         if (live) {
-          target = p.kept_target[row];
-          target = target >= p.v0 ? target - p.v0 : -1;
-          lse2 = p.lse2[row];
-          weight_of = p.weight_of[row];
+          lse2 = p.lse2[p.first_row + row];
+          weight_of = p.weight_of[p.first_row + row];
         }
       }
       if (!mbar_wait(&done[buffer], buffer_phase, &abort_flag)) break;
       tcgen05_fence_after();
       const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + buffer * kTileN + half * (kTileN / 2);
-      if constexpr (PASS == kStats) {
+      if constexpr (PASS == kStats || PASS == kCodes) {
+        // The half tile's maximum first: sums and codes count from it.
         float top = -INFINITY, sum = 0.f;
 #pragma unroll 1
         for (int c = 0; c < kTileN / 2 && column + c < p.vn; c += 32) {
           uint32_t r[32];
           tmem_load_32(src + c, r);
-          float y[32], high = top;
           const int valid = p.vn - column - c;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            y[e] = e < valid ? __uint_as_float(r[e]) * to_log2 : -INFINITY;
-            high = fmaxf(high, y[e]);
+          for (int e = 0; e < 32; ++e)
+            top = fmaxf(top, e < valid ? __uint_as_float(r[e]) * to_log2 : -INFINITY);
+        }
+        const float pivot = top == -INFINITY ? 0.f : top;
+        const bool rows_exist = first_row < p.row_limit;
+#pragma unroll 1
+        for (int c = 0; c < kTileN / 2 && column + c < p.vn; c += 64) {
+          if constexpr (PASS == kCodes) {
+            if (lane == 0) tensor_store_wait_read();
+            __syncwarp();
           }
-          const int at = target - column - c;
-          if (at >= 0 && at < 32) {
-            float z = y[0];
 #pragma unroll
-            for (int e = 1; e < 32; ++e) z = at == e ? y[e] : z;
-            p.target_logit[p.first_row + row] = z;
+          for (int h = 0; h < 2; ++h) {
+            uint32_t r[32];
+            tmem_load_32(src + c + h * 32, r);
+            const int valid = p.vn - column - c - h * 32, at = target - column - c - h * 32;
+            if (at >= 0 && at < 32) {
+              float z = __uint_as_float(r[0]);
+#pragma unroll
+              for (int e = 1; e < 32; ++e) z = at == e ? __uint_as_float(r[e]) : z;
+              p.target_logit[p.first_row + row] = z * to_log2;
+            }
+            float part = 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float down = fmaf(__uint_as_float(r[e]), to_log2, -pivot);  // at most zero
+              part += e < valid ? exp2_approx(down) : 0.f;
+              if constexpr (PASS == kCodes) {
+                // Adding 2^23 leaves the rounded integer in the low bits.
+                const float code = fminf(fmaf(down, -kCodeSteps, 8388608.f), 8388608.f + 65535.f);
+                r[e] = live ? __float_as_uint(code) : 0u;
+              }
+            }
+            sum += part;
+            if constexpr (PASS == kCodes) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                store_shared16(block_slot(staging, lane, h * 4 + q),
+                               __byte_perm(r[8 * q], r[8 * q + 1], 0x5410),
+                               __byte_perm(r[8 * q + 2], r[8 * q + 3], 0x5410),
+                               __byte_perm(r[8 * q + 4], r[8 * q + 5], 0x5410),
+                               __byte_perm(r[8 * q + 6], r[8 * q + 7], 0x5410));
+            }
           }
-          // A row of nothing but -inf so far: subtract zero, its terms are exp2(-inf) = 0.
-          const float pivot = high == -INFINITY ? 0.f : high;
-          float part = 0.f;
-#pragma unroll
-          for (int e = 0; e < 32; ++e) part += exp2_approx(y[e] - pivot);
-          sum = fmaf(sum, exp2_approx(top - pivot), part);
-          top = high;
+          if constexpr (PASS == kCodes) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0 && rows_exist) tensor_store_2d(&map_2, column + c, first_row, staging);
+          }
         }
         if (live)
           p.partials[(int64_t)row * (2 * order.tiles_n) + 2 * (t.n / kTileN) + half] =
@@ -555,9 +604,15 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
           __syncwarp();
           if (lane == 0 && rows_exist) tensor_store_2d(&map_2, column + c, first_row, staging);
         }
-      } else if (!t.weight && p.slices_out != nullptr) {
-        // A slice of dH: FP32, added to the others by loss_slices_kernel.
-        const int64_t place = ((int64_t)(p.first_slice + t.slice) * p.N + row) * p.D + column;
+      } else if ((t.weight ? p.weight_out : p.slices_out) != nullptr) {
+        // A part of the sum: FP32, added to the others by loss_slices_kernel.
+        int64_t place = -1;
+        if (t.weight) {
+          if (row < p.vn) place = (int64_t)(p.v0 + row) * p.D + column;
+        } else if (row < kept) {
+          place = ((int64_t)(p.first_slice + t.slice) * p.N + row) * p.D + column;
+        }
+        float* parts = t.weight ? p.weight_out : p.slices_out;
 #pragma unroll 1
         for (int c = 0; c < kTileN / 2 && column + c < p.D; c += 32) {
           uint32_t r[32];
@@ -570,15 +625,14 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
             else
               store_shared16(block_slot(staging, lane, q), 0u, 0u, 0u, 0u);
           }
-          write_block<float>(staging, p.slices_out + c, row < kept ? place : -1, p.D - column - c,
-                             p.D % 4 == 0, lane);
+          write_block<float>(staging, parts + c, place, p.D - column - c, p.D % 4 == 0, lane);
         }
       } else {
         int64_t place = -1;
         if (t.weight) {
           if (row < p.vn) place = (int64_t)(p.v0 + row) * p.D + column;
         } else if (row < kept) {
-          place = (int64_t)p.kept_index[row] * p.D + column;
+          place = (int64_t)p.kept_index[p.first_row + row] * p.D + column;
         }
         T* out = static_cast<T*>(t.weight ? p.dweight : p.dhidden);
         const bool vector = t.weight ? p.vector_dweight : p.vector_dhidden;
@@ -611,7 +665,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
       buffer ^= 1;
       if (buffer == 0) buffer_phase ^= 1u;
     }
-    if (PASS == kProbs && lane == 0) tensor_store_wait_read();
+    if ((PASS == kProbs || PASS == kCodes) && lane == 0) tensor_store_wait_read();
   }
   __syncwarp();
   tcgen05_fence_before();
@@ -629,19 +683,21 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
   if constexpr (PAIR) cluster_barrier();
 }
 
-// dH from its slices, added in order; one warp a kept row.
+// A gradient from its parts, added in order; one warp a row.  dH: the kept rows, to their places in
+// the input.  dW (no `kept_index`): rows as they are.
 template <typename T>
 __global__ void __launch_bounds__(256)
 loss_slices_kernel(const float* __restrict__ slices, int count, const int32_t* kept_rows,
                    const int32_t* __restrict__ kept_index, const float* gradient_scale, float scale,
                    int64_t N, int D, T* out, int vector) {
   const float out_scale = scale * *gradient_scale * (__is_same(T, __half) ? 1.f / kHalfLift : 1.f);
-  const int lane = threadIdx.x & 31, kept = *kept_rows;
+  const int lane = threadIdx.x & 31;
+  const int64_t kept = kept_index != nullptr ? *kept_rows : N;
   const int64_t all = N * D;
   for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < kept;
        row += (int64_t)gridDim.x * 8) {
     const float* mine = slices + row * D;
-    T* to = out + (int64_t)kept_index[row] * D;
+    T* to = out + (kept_index != nullptr ? kept_index[row] : row) * D;
     if (vector) {
 #pragma unroll 2
       for (int c = lane * 8; c < D; c += 256) {
@@ -679,39 +735,93 @@ loss_slices_kernel(const float* __restrict__ slices, int count, const int32_t* k
 
 // ------------------------------------------------------------------------------ joining the loss
 
-// One warp per kept row: log2 of the row's sum of exponentials from its (max, sum) pairs.
-__global__ void __launch_bounds__(256)
-loss_join_kernel(const float2* __restrict__ partials, int pairs, const int32_t* count, int first_row,
-                 int row_limit, const float* __restrict__ target_logit,
-                 const int32_t* __restrict__ kept_index, float* __restrict__ lse2,
-                 float* __restrict__ losses) {
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= row_limit || first_row + row >= *count) return;
-  const float2* mine = partials + (int64_t)row * pairs;
-  float top = -INFINITY, sum = 0.f;
-#pragma unroll 4
-  for (int i = lane; i < pairs; i += 32) {
-    const float2 v = mine[i];
-    const float high = fmaxf(top, v.x), pivot = high == -INFINITY ? 0.f : high;
-    sum = sum * exp2f(top - pivot) + v.y * exp2f(v.x - pivot);
-    top = high;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float other_top = __shfl_xor_sync(0xffffffffu, top, o);
-    const float other_sum = __shfl_xor_sync(0xffffffffu, sum, o);
+constexpr int kJoinThreads = 256;
+
+// log2 of a row's sum of exponentials from its (max, sum) pairs, by one CTA, in a fixed order: the
+// loss is the same bits whether its gradients are formed beside it or not.
+struct RowJoin {
+  float top, sum;
+  __device__ __forceinline__ void add(float other_top, float other_sum) {
     const float high = fmaxf(top, other_top), pivot = high == -INFINITY ? 0.f : high;
     sum = sum * exp2f(top - pivot) + other_sum * exp2f(other_top - pivot);
     top = high;
   }
-  if (lane == 0) {
+};
+
+__device__ __forceinline__ float join_row(const float2* mine, int pairs, float at_target) {
+  __shared__ RowJoin parts[kJoinThreads / 32];
+  const int tid = threadIdx.x;
+  RowJoin row{-INFINITY, 0.f};
+  for (int i = tid; i < pairs; i += kJoinThreads) {
+    const float2 v = __ldcg(mine + i);
+    row.add(v.x, v.y);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    row.add(__shfl_xor_sync(0xffffffffu, row.top, o), __shfl_xor_sync(0xffffffffu, row.sum, o));
+  __syncthreads();  // the previous row's use of `parts` is over
+  if ((tid & 31) == 0) parts[tid >> 5] = row;
+  __syncthreads();
+  row = parts[0];
+#pragma unroll
+  for (int w = 1; w < kJoinThreads / 32; ++w) row.add(parts[w].top, parts[w].sum);
+  // No logit at the target (an id outside the vocabulary): the loss and the gradients of the
+  // row are not numbers, so the mistake shows.
+  return isnan(at_target) ? at_target : row.top + log2f(row.sum);
+}
+
+// One CTA a kept row: its normaliser and its loss.
+__global__ void __launch_bounds__(kJoinThreads)
+loss_join_kernel(const float2* __restrict__ partials, int pairs, const int32_t* count, int first_row,
+                 int row_limit, const float* __restrict__ target_logit,
+                 const int32_t* __restrict__ kept_index, float* __restrict__ lse2,
+                 float* __restrict__ losses) {
+  const int rows = min(max(*count - first_row, 0), row_limit);
+  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
     const float at_target = target_logit[first_row + row];
-    // No logit at the target (an id outside the vocabulary): the loss and the gradients of the
-    // row are not numbers, so the mistake shows.
-    float joined = top + log2f(sum);
-    if (isnan(at_target)) joined = at_target;
-    lse2[first_row + row] = joined;
-    losses[kept_index[first_row + row]] = (joined - at_target) * kLn2;
+    const float joined = join_row(partials + (int64_t)row * pairs, pairs, at_target);
+    if (threadIdx.x == 0) {
+      lse2[first_row + row] = joined;
+      losses[kept_index[first_row + row]] = (joined - at_target) * kLn2;
+    }
+  }
+}
+
+// The same, and the row's codes become P = p - [v = target] in place.
+__global__ void __launch_bounds__(kJoinThreads)
+loss_probs_kernel(const float2* __restrict__ partials, int pairs, const int32_t* count, int first_row,
+                  int row_limit, const float* __restrict__ target_logit,
+                  const int32_t* __restrict__ kept_target, const int32_t* __restrict__ kept_index,
+                  float* __restrict__ losses, unsigned short* codes, int64_t stride, int V) {
+  const int tid = threadIdx.x, rows = min(max(*count - first_row, 0), row_limit);
+  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+    const float2* mine = partials + (int64_t)row * pairs;
+    const float at_target = target_logit[first_row + row];
+    const float lse2 = join_row(mine, pairs, at_target);
+    if (tid == 0) losses[kept_index[first_row + row]] = (lse2 - at_target) * kLn2;
+    const int target = kept_target[first_row + row];
+    const float residue = exp2f(at_target - lse2) - 1.f;
+    uint4* chunks = reinterpret_cast<uint4*>(codes + (int64_t)row * stride);
+#pragma unroll 4
+    for (int c = tid; c < (V + 7) / 8; c += kJoinThreads) {
+      const uint4 raw = __ldcs(chunks + c);
+      const float base = __ldcg(&mine[c >> 4].x) - lse2;  // sixteen chunks to a half tile
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+      uint32_t out[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        // 2^23 + code as a float, then minus 2^23: exact
+        const float lo = __uint_as_float(__byte_perm(w[k], 0x4b000000u, 0x7610)) - 8388608.f;
+        const float hi = __uint_as_float(__byte_perm(w[k], 0x4b000000u, 0x7632)) - 8388608.f;
+        float p0 = exp2_approx(fmaf(lo, -1.f / kCodeSteps, base));
+        float p1 = exp2_approx(fmaf(hi, -1.f / kCodeSteps, base));
+        const int column = c * 8 + 2 * k;
+        if (column == target) p0 = residue;
+        if (column + 1 == target) p1 = residue;
+        out[k] = pack_bf16x2(p0, p1);
+      }
+      chunks[c] = make_uint4(out[0], out[1], out[2], out[3]);
+    }
   }
 }
 
@@ -732,6 +842,25 @@ loss_reduce_kernel(const float* __restrict__ losses, int64_t N, const int32_t* c
     for (int w = 0; w < 32; ++w) total += sums[w];
     *out = (float)(mean ? total / (double)*count : total);  // no kept row: not a number
   }
+}
+
+// Gradients for an upstream gradient of one, times the one that came: eight elements a thread.
+__global__ void __launch_bounds__(256)
+loss_scale_kernel(const __nv_bfloat16* __restrict__ in, const float* upstream, int64_t elements,
+                  __nv_bfloat16* __restrict__ out) {
+  const float g = *upstream;
+  const int64_t chunks = elements / 8, stride = (int64_t)gridDim.x * 256;
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+#pragma unroll 4
+  for (int64_t i = first; i < chunks; i += stride) {
+    float f[8];
+    unpack8(__ldcs(reinterpret_cast<const uint4*>(in) + i), f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= g;
+    reinterpret_cast<uint4*>(out)[i] = pack8(f);
+  }
+  for (int64_t i = chunks * 8 + first; i < elements; i += stride)
+    out[i] = __float2bfloat16_rn(__bfloat162float(in[i]) * g);
 }
 
 // ------------------------------------------------------------------------------ before the gradients

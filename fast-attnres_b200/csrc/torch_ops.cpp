@@ -321,43 +321,85 @@ Tensor embed(const Tensor& tokens, const Tensor& table, const optional<Tensor>& 
 
 constexpr int64_t kAlign = 64;  // elements between the arrays that share one allocation
 
-// -> loss, kept rows, their [2, N] indices and targets, their count, log2 of their sums
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> loss_forward(
-    const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignored,
-    int64_t reduction, double scale) {
+struct LossForward {
+  Tensor loss, kept, index, count, sums, dhidden, dweight;
+};
+
+LossForward run_loss(const Tensor& hidden, const Tensor& weight, const Tensor& targets,
+                     int64_t ignored, int64_t reduction, double scale, bool gradients,
+                     bool need_hidden, bool need_weight) {
   const int64_t width = hidden.size(-1), vocabulary = weight.size(0), rows = hidden.numel() / width;
   const auto floats = hidden.options().dtype(at::kFloat);
   const auto ints = hidden.options().dtype(at::kInt);
   const bool each = reduction == ATTNRES_B200_LOSS_NONE;
-  Tensor kept = at::empty({rows, (width + 7) / 8 * 8}, hidden.options());
-  Tensor index = at::empty({2, rows}, ints), count = at::empty({1}, ints);
-  Tensor sums = at::empty({rows}, floats);
-  Tensor loss = each ? at::empty(targets.sizes(), floats) : at::empty({}, floats);
+  LossForward r;
+  r.kept = at::empty({rows, (width + 7) / 8 * 8}, hidden.options());
+  r.index = at::empty({2, rows}, ints);
+  r.count = at::empty({1}, ints);
+  if (!gradients) r.sums = at::empty({rows}, floats);
+  r.loss = each ? at::empty(targets.sizes(), floats) : at::empty({}, floats);
+  if (gradients && need_hidden) r.dhidden = at::empty(hidden.sizes(), hidden.options());
+  if (gradients && need_weight)
+    r.dweight = rows ? at::empty({vocabulary, width}, hidden.options())
+                     : at::zeros({vocabulary, width}, hidden.options());
   if (rows == 0) {
-    count.zero_();
+    r.count.zero_();
     if (!each)
-      loss.fill_(reduction == ATTNRES_B200_LOSS_SUM ? 0.0 : std::numeric_limits<double>::quiet_NaN());
-    return {loss, kept, index, count, sums};
+      r.loss.fill_(reduction == ATTNRES_B200_LOSS_SUM ? 0.0
+                                                      : std::numeric_limits<double>::quiet_NaN());
+    return r;
   }
   c10::cuda::CUDAGuard guard(hidden.device());
   const Rows source = rows_of(hidden), head = rows_of(weight);
   const Tensor ids = targets.contiguous();
   const int64_t bytes = sized(
-      attnres_b200_loss_workspace_bytes(rows, (int32_t)vocabulary, (int32_t)width, 0),
+      attnres_b200_loss_workspace_bytes(
+          rows, (int32_t)vocabulary, (int32_t)width,
+          gradients ? ATTNRES_B200_LOSS_FORWARD_GRADIENTS : ATTNRES_B200_LOSS_FORWARD),
       "attnres_b200_loss_workspace_bytes");
   const int64_t losses_bytes = each ? 0 : (rows + kAlign) / kAlign * kAlign * 4;
   Tensor workspace = at::empty({bytes + losses_bytes}, hidden.options().dtype(at::kByte));
   char* space = static_cast<char*>(workspace.data_ptr());
-  float* losses = each ? loss.data_ptr<float>() : reinterpret_cast<float*>(space);
+  float* losses = each ? r.loss.data_ptr<float>() : reinterpret_cast<float*>(space);
   check(attnres_b200_loss_forward(
             source.kept.data_ptr(), source.stride, head.kept.data_ptr(), head.stride, ids.data_ptr(),
             ids.scalar_type() == at::kLong, rows, (int32_t)vocabulary, (int32_t)width,
             type_code(hidden.scalar_type()), ignored, (float)scale, (int32_t)reduction,
-            kept.data_ptr(), index.data_ptr<int32_t>(), index.data_ptr<int32_t>() + rows,
-            count.data_ptr<int32_t>(), sums.data_ptr<float>(), losses,
-            each ? nullptr : loss.data_ptr<float>(), space + losses_bytes, bytes, stream_of(hidden)),
+            r.kept.data_ptr(), r.index.data_ptr<int32_t>(), r.index.data_ptr<int32_t>() + rows,
+            r.count.data_ptr<int32_t>(), static_cast<float*>(pointer(r.sums)), losses,
+            each ? nullptr : r.loss.data_ptr<float>(), pointer(r.dhidden), pointer(r.dweight),
+            space + losses_bytes, bytes, stream_of(hidden)),
         "attnres_b200_loss_forward");
-  return {loss, kept, index, count, sums};
+  return r;
+}
+
+// -> loss, kept rows, their [2, N] indices and targets, their count, log2 of their sums
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> loss_forward(
+    const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignored,
+    int64_t reduction, double scale) {
+  LossForward r = run_loss(hidden, weight, targets, ignored, reduction, scale, false, false, false);
+  return {r.loss, r.kept, r.index, r.count, r.sums};
+}
+
+// -> loss, and the gradients of hidden and weight for an upstream gradient of one
+std::tuple<Tensor, Tensor, Tensor> loss_with_gradients(const Tensor& hidden, const Tensor& weight,
+                                                       const Tensor& targets, int64_t ignored,
+                                                       int64_t reduction, double scale,
+                                                       bool need_hidden, bool need_weight) {
+  LossForward r = run_loss(hidden, weight, targets, ignored, reduction, scale, true, need_hidden,
+                           need_weight);
+  return {r.loss, or_nothing(r.dhidden, hidden, hidden.scalar_type()),
+          or_nothing(r.dweight, hidden, hidden.scalar_type())};
+}
+
+Tensor loss_scale_gradient(const Tensor& gradient, const Tensor& upstream) {
+  Tensor out = at::empty(gradient.sizes(), gradient.options());
+  if (gradient.numel() == 0) return out;
+  c10::cuda::CUDAGuard guard(gradient.device());
+  check(attnres_b200_loss_scale_gradient(gradient.data_ptr(), upstream.data_ptr<float>(),
+                                         gradient.numel(), out.data_ptr(), stream_of(gradient)),
+        "attnres_b200_loss_scale_gradient");
+  return out;
 }
 
 std::tuple<Tensor, Tensor> loss_backward(const Tensor& grad, const Tensor& weight,
@@ -380,7 +422,8 @@ std::tuple<Tensor, Tensor> loss_backward(const Tensor& grad, const Tensor& weigh
     const Rows head = rows_of(weight);
     const Tensor ids = targets.contiguous(), upstream = grad.contiguous();
     const int64_t bytes = sized(
-        attnres_b200_loss_workspace_bytes(rows, (int32_t)vocabulary, (int32_t)width, 1),
+        attnres_b200_loss_workspace_bytes(rows, (int32_t)vocabulary, (int32_t)width,
+                                          ATTNRES_B200_LOSS_BACKWARD),
         "attnres_b200_loss_workspace_bytes");
     Tensor workspace = at::empty({bytes}, weight.options().dtype(at::kByte));
     check(attnres_b200_loss_backward(
@@ -396,35 +439,62 @@ std::tuple<Tensor, Tensor> loss_backward(const Tensor& grad, const Tensor& weigh
           or_nothing(dweight, weight, weight.scalar_type())};
 }
 
+// Which of the two forwards serves a call that will be differentiated.
+bool gradients_in_forward(const Tensor& hidden, int64_t reduction) {
+  return attnres_b200_loss_gradients_in_forward((int32_t)hidden.size(-1),
+                                                type_code(hidden.scalar_type()),
+                                                (int32_t)reduction) != 0;
+}
+
 struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
   static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight,
                         const Tensor& targets, int64_t ignored, int64_t reduction, double scale) {
+    const bool need_hidden = hidden.requires_grad(), need_weight = weight.requires_grad();
+    ctx->set_materialize_grads(false);
+    at::AutoDispatchBelowADInplaceOrView below;
+    const bool early = (need_hidden || need_weight) && gradients_in_forward(hidden, reduction);
+    ctx->saved_data["early"] = early;
+    if (early) {
+      static auto op = operation<decltype(loss_with_gradients)>(
+          "attnres_b200::linear_cross_entropy_with_gradients");
+      auto [loss, dhidden, dweight] =
+          op.call(hidden, weight, targets, ignored, reduction, scale, need_hidden, need_weight);
+      ctx->save_for_backward({dhidden, dweight});
+      return loss;
+    }
     static auto op =
         operation<decltype(loss_forward)>("attnres_b200::linear_cross_entropy_forward");
-    at::AutoDispatchBelowADInplaceOrView below;
     auto [loss, kept, index, count, sums] =
         op.call(hidden, weight, targets, ignored, reduction, scale);
     ctx->save_for_backward({weight, targets, kept, index, count, sums});
     ctx->saved_data["ignored"] = ignored;
     ctx->saved_data["reduction"] = reduction;
     ctx->saved_data["scale"] = scale;
-    ctx->set_materialize_grads(false);
     return loss;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return variable_list(6);
-    static auto op =
-        operation<decltype(loss_backward)>("attnres_b200::linear_cross_entropy_backward");
     const auto saved = ctx->get_saved_variables();
     auto& data = ctx->saved_data;
     const bool nh = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [dhidden, dweight] =
-        op.call(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4], saved[5],
-                data["ignored"].toInt(), data["reduction"].toInt(), data["scale"].toDouble(), nh, nw);
-    return once({nh ? dhidden : Tensor(), nw ? dweight : Tensor(), Tensor(), Tensor(), Tensor(),
-                 Tensor()});
+    Tensor dhidden, dweight;
+    if (data["early"].toBool()) {
+      static auto op = operation<decltype(loss_scale_gradient)>(
+          "attnres_b200::linear_cross_entropy_scale_gradient");
+      if (nh) dhidden = op.call(saved[0], grads[0]);
+      if (nw) dweight = op.call(saved[1], grads[0]);
+    } else {
+      static auto op =
+          operation<decltype(loss_backward)>("attnres_b200::linear_cross_entropy_backward");
+      auto [dh, dw] = op.call(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4], saved[5],
+                              data["ignored"].toInt(), data["reduction"].toInt(),
+                              data["scale"].toDouble(), nh, nw);
+      if (nh) dhidden = dh;
+      if (nw) dweight = dw;
+    }
+    return once({dhidden, dweight, Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
@@ -454,6 +524,10 @@ TORCH_LIBRARY_FRAGMENT(attnres_b200, m) {
         "ScalarType type) -> Tensor");
   m.def("linear_cross_entropy_forward(Tensor hidden, Tensor weight, Tensor targets, int ignored, "
         "int reduction, float scale) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("linear_cross_entropy_with_gradients(Tensor hidden, Tensor weight, Tensor targets, "
+        "int ignored, int reduction, float scale, bool need_hidden, bool need_weight) "
+        "-> (Tensor, Tensor, Tensor)");
+  m.def("linear_cross_entropy_scale_gradient(Tensor gradient, Tensor upstream) -> Tensor");
   m.def("linear_cross_entropy_backward(Tensor grad, Tensor weight, Tensor targets, Tensor kept, "
         "Tensor index, Tensor count, Tensor sums, int ignored, int reduction, float scale, "
         "bool need_hidden, bool need_weight) -> (Tensor, Tensor)");
@@ -469,6 +543,8 @@ TORCH_LIBRARY_IMPL(attnres_b200, CUDA, m) {
   m.impl("embedding_backward", embedding_backward_sym);
   m.impl("embed", embed);
   m.impl("linear_cross_entropy_forward", loss_forward);
+  m.impl("linear_cross_entropy_with_gradients", loss_with_gradients);
+  m.impl("linear_cross_entropy_scale_gradient", loss_scale_gradient);
   m.impl("linear_cross_entropy_backward", loss_backward);
   m.impl("linear_cross_entropy", loss);
 }

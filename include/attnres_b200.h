@@ -379,31 +379,45 @@ int attnres_b200_embedding_backward(
  *   count            device int32 [1], how many there are
  *   lse2             device FP32 [N]: log2 of each kept row's sum of exponentials
  *
+ * Gradients in the forward: with `dhidden` or `dweight` given (BF16, _SUM or _MEAN only; `lse2` may
+ * then be NULL) the forward also writes the gradients for an upstream gradient of one, from the same
+ * logits; attnres_b200_loss_scale_gradient multiplies them by the one that comes.
+ * attnres_b200_loss_gradients_in_forward says where that is faster than the backward, which forms
+ * the logits a second time.  It costs the forward of a loss that is never differentiated as much as
+ * a backward.
+ *
  *   upstream         device FP32: [N] with stride `upstream_stride` for _NONE, else one number
  *   dhidden          device [N,D] of `type`, contiguous; dweight [V,D], contiguous; either may be
  *                    NULL
- *   workspace        16-byte aligned, attnres_b200_loss_workspace_bytes(N, V, D, backward) bytes
+ *   workspace        16-byte aligned, attnres_b200_loss_workspace_bytes(N, V, D, pass) bytes, `pass`
+ *                    one of the three below
  *
- * The backward forms the logits a second time, a piece of the vocabulary after the other, so
- * neither pass holds more of [N,V] than one piece (512 MiB, or 4096 ids where that is more).
- * Results are the same bits every time.
+ * No pass holds more of [N,V] than one piece, 16 bits an element: 1 GiB, or 4096 ids (backward) or
+ * 1024 rows (forward with gradients) where that is more.  Results are the same bits every time.
  */
 #define ATTNRES_B200_LOSS_NONE 0
 #define ATTNRES_B200_LOSS_SUM 1
 #define ATTNRES_B200_LOSS_MEAN 2
-int64_t attnres_b200_loss_workspace_bytes(int64_t N, int32_t V, int32_t D, int32_t backward);
+#define ATTNRES_B200_LOSS_FORWARD 0
+#define ATTNRES_B200_LOSS_BACKWARD 1
+#define ATTNRES_B200_LOSS_FORWARD_GRADIENTS 2
+int64_t attnres_b200_loss_workspace_bytes(int64_t N, int32_t V, int32_t D, int32_t pass);
+int32_t attnres_b200_loss_gradients_in_forward(int32_t D, int32_t type, int32_t reduction);
 int attnres_b200_loss_forward(
     const void* hidden, int64_t hidden_row_stride, const void* weight, int64_t weight_row_stride,
     const void* targets, int32_t targets_64, int64_t N, int32_t V, int32_t D, int32_t type,
     int64_t ignored, float scale, int32_t reduction, void* kept, int32_t* kept_index,
-    int32_t* kept_target, int32_t* count, float* lse2, float* losses, float* loss, void* workspace,
-    int64_t workspace_bytes, void* stream);
+    int32_t* kept_target, int32_t* count, float* lse2, float* losses, float* loss, void* dhidden,
+    void* dweight, void* workspace, int64_t workspace_bytes, void* stream);
 int attnres_b200_loss_backward(
     const float* upstream, int64_t upstream_stride, const void* weight, int64_t weight_row_stride,
     const void* targets, int32_t targets_64, int64_t N, int32_t V, int32_t D, int32_t type,
     int64_t ignored, float scale, int32_t reduction, const void* kept, const int32_t* kept_index,
     const int32_t* kept_target, const int32_t* count, const float* lse2, void* dhidden,
     void* dweight, void* workspace, int64_t workspace_bytes, void* stream);
+/* out = gradient * *upstream: BF16, `elements` of them, both 16-byte aligned. */
+int attnres_b200_loss_scale_gradient(const void* gradient, const float* upstream, int64_t elements,
+                                     void* out, void* stream);
 
 /*
  * Diagnostics (no counterpart in the reference).  The TMA-staged kernels bound

@@ -145,16 +145,20 @@ def test_loss_entry_points_check_their_arguments():
     lib = _native.load()
 
     def forward(N=3, V=7, D=16, kind=0, scale=1.0, reduction=2, hidden=0x1000, weight=0x2000,
-                targets=0x3000, kept=0x4000, loss=0x5000, workspace=0x6000, size=1 << 40):
+                targets=0x3000, kept=0x4000, loss=0x5000, workspace=0x6000, size=1 << 40, sums=0x7300,
+                dh=None, dw=None):
         return lib.attnres_b200_loss_forward(hidden, D, weight, D, targets, 1, N, V, D, kind, -100,
-                                             scale, reduction, kept, 0x7000, 0x7100, 0x7200, 0x7300,
-                                             0x7400, loss, workspace, size, None)
+                                             scale, reduction, kept, 0x7000, 0x7100, 0x7200, sums,
+                                             0x7400, loss, dh, dw, workspace, size, None)
 
     assert forward(N=0) == 5 and forward(D=8193) == 3 and forward(V=0) == 14
     assert forward(kind=2) == 13 and forward(scale=float("inf")) == 6 and forward(reduction=3) == 10
     assert forward(hidden=None) == 1 and forward(kept=None) == 1 and forward(loss=None) == 1
     assert forward(hidden=0x1001) == 7 and forward(kept=0x4008) == 7 and forward(targets=0x3004) == 7
-    assert forward(size=16) == 8
+    assert forward(size=16) == 8 and forward(sums=None) == 1
+    # gradients in the forward: BF16 and one loss
+    assert forward(dh=0x8000, kind=1) == 13 and forward(dw=0x8000, reduction=0) == 10
+    assert forward(dh=0x8001) == 7 and forward(dh=0x8000, sums=None, size=16) == 8
 
     def backward(dh=0x1000, dw=0x2000, upstream=0x3000, workspace=0x6000, size=1 << 40, kind=0):
         return lib.attnres_b200_loss_backward(upstream, 1, 0x2000, 16, 0x3000, 1, 3, 7, 16, kind,
@@ -167,4 +171,15 @@ def test_loss_entry_points_check_their_arguments():
     assert lib.attnres_b200_loss_workspace_bytes(0, 7, 16, 0) == -5
     assert lib.attnres_b200_loss_workspace_bytes(3, 0, 16, 1) == -14
     # a piece of the vocabulary, not the vocabulary: 16 384 x 128 000 logits would be 4 GB
-    assert lib.attnres_b200_loss_workspace_bytes(16384, 128000, 64, 1) < 600 << 20
+    assert lib.attnres_b200_loss_workspace_bytes(16384, 128000, 64, 1) < 1200 << 20
+    assert lib.attnres_b200_loss_workspace_bytes(16384, 128000, 64, 2) < 1300 << 20
+    assert lib.attnres_b200_loss_workspace_bytes(3, 7, 16, 3) == -10
+    policy = lib.attnres_b200_loss_gradients_in_forward
+    assert policy(512, 0, 2) and policy(1024, 0, 1)
+    assert not policy(511, 0, 2) and not policy(1024, 1, 2) and not policy(1024, 0, 0)
+
+    def scaled(gradient=0x1000, upstream=0x2000, count=8, out=0x3000):
+        return lib.attnres_b200_loss_scale_gradient(gradient, upstream, count, out, None)
+
+    assert scaled(count=0) == 5 and scaled(gradient=None) == 1 and scaled(upstream=None) == 1
+    assert scaled(gradient=0x1008) == 7 and scaled(out=0x3002) == 7

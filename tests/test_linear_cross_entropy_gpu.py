@@ -10,6 +10,10 @@ Tolerances, with e = 2^-23 (a step of FP32) and h half a step of the inputs' typ
 FP16 keeps P as 2^15 P / max c: half of its smallest subnormal is 2^-40 max c in P.
 BF16 keeps P / max c, and the exponential of a logit that lies more than 126 powers of two below the
 row's sum is zero (FP32 has no normal number for it): 2^-126 max c in P, whatever P's own size.
+Where the forward forms the gradients (BF16, a sum or mean, 512 features and more) a logit passes
+through a code in steps of 2^-11 powers of two below its half tile's maximum, 65535 of them at most:
+a probability is off by a factor 2^(+-2^-12), less than 2^-12, or is 2^-32 of that maximum instead of
+something smaller; and the gradient is rounded once more when the upstream gradient multiplies it.
 """
 import math
 
@@ -58,15 +62,22 @@ def _reference(hidden, weight, targets, reduction, scale, upstream, ignore_index
     p = (z - lse[:, None]).exp()
     cp = (2 * cz + 8 * E * (1 + lse.abs()))[:, None]
     spread = c.abs() * p * cp
+    early = hidden.dtype == BF16 and reduction != "none" and width >= 512
+    if early:
+        spread += c.abs() * (2.0**-12 * p + 2.0**-32)
     p.scatter_add_(1, ids[:, None], torch.full_like(p[:, :1], -1.0))
     p *= c
     spread += half * p.abs()
     spread += (2.0**-40 if hidden.dtype == FP16 else 2.0**-126) * c.abs().max() * kept[:, None]
     size = p.abs() + spread
+    dhidden, dweight = p @ w, p.t() @ h
+    again = half if early else 0.0
     return dict(
         loss=(loss, slack),
-        dhidden=(p @ w, spread @ w.abs() + (vocabulary / 8 + 24) * E * (size @ w.abs())),
-        dweight=(p.t() @ h, spread.t() @ h.abs() + (rows / 8 + 24) * E * (size.t() @ h.abs())))
+        dhidden=(dhidden, again * dhidden.abs() + (1 + again) * (
+            spread @ w.abs() + (vocabulary / 8 + 24) * E * (size @ w.abs()))),
+        dweight=(dweight, again * dweight.abs() + (1 + again) * (
+            spread.t() @ h.abs() + (rows / 8 + 24) * E * (size.t() @ h.abs()))))
 
 
 def _inside(got, want, slack, what):
@@ -222,6 +233,56 @@ def test_linear_cross_entropy_upstream_weights_of_any_size(dtype):
     assert not any(g.any() for g in _check(hidden, weight, targets, reduction="none", upstream=zero)[1:])
 
 
+@pytest.mark.parametrize("width", [96, 640])
+def test_linear_cross_entropy_upstream_of_one_number(width):
+    hidden, weight, targets = _case(200, 300, width, BF16, ignored=0.2, seed=15)
+    for upstream in (1.0, 0.3, -7.0, 0.0):
+        _check(hidden, weight, targets, upstream=torch.tensor(upstream, device="cuda"))
+    for upstream in (float("inf"), float("nan")):
+        from attnres.loss import linear_cross_entropy
+        loss = linear_cross_entropy(hidden, weight, targets)
+        grads = torch.autograd.grad(loss, (hidden, weight), torch.tensor(upstream, device="cuda"))
+        assert not any(g.isfinite().all() for g in grads)
+
+
+@pytest.mark.parametrize("width", [96, 640])
+def test_linear_cross_entropy_backward_twice_through_one_forward(width):
+    from attnres.loss import linear_cross_entropy
+    hidden, weight, targets = _case(200, 300, width, BF16, ignored=0.2, seed=16)
+    leaves = [hidden.requires_grad_(), weight.requires_grad_()]
+    loss = linear_cross_entropy(hidden, weight, targets)
+    first = torch.autograd.grad(loss, leaves, torch.tensor(2.0, device="cuda"), retain_graph=True)
+    second = torch.autograd.grad(loss, leaves)
+    assert all(torch.equal(a, 2 * b) for a, b in zip(first, second))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_linear_cross_entropy_wide_rows_special_cases(reduction):
+    """The cases above that are narrow, where the forward forms the gradients."""
+    from attnres.loss import linear_cross_entropy
+    hidden, weight, targets = _case(140, 300, 520, BF16, seed=17)
+    leaves = [hidden.requires_grad_(), weight.requires_grad_()]
+    loss = linear_cross_entropy(hidden, weight, torch.full_like(targets, -100), reduction=reduction)
+    assert loss.isnan() if reduction == "mean" else not loss.any()
+    assert not any(g.any() for g in torch.autograd.grad(loss, leaves))
+    bad = targets.clone()
+    bad[3] = 300
+    loss = linear_cross_entropy(*leaves, bad, reduction=reduction)
+    dhidden, dweight = torch.autograd.grad(loss, leaves)
+    assert loss.isnan() and dhidden[3].isnan().all() and dweight.isnan().all()
+    assert dhidden[:3].isfinite().all() and dhidden[4:].isfinite().all()
+    drop = torch.arange(140, device="cuda") % 3 == 0
+    masked = torch.where(drop, -100, targets)
+    results = []
+    for filler in (0.0, float("nan"), float("inf")):
+        dirty = torch.where(drop[:, None], torch.tensor(filler, dtype=BF16, device="cuda"), hidden.detach())
+        pair = [dirty.requires_grad_(), weight]
+        loss = linear_cross_entropy(*pair, masked, reduction=reduction)
+        results.append([loss.detach(), *torch.autograd.grad(loss, pair)])
+    assert all(torch.equal(a, b) for other in results[1:] for a, b in zip(results[0], other))
+    _check(hidden.detach(), weight.detach(), targets, reduction=reduction, scale=300.0)
+
+
 def test_linear_cross_entropy_strange_upstream_weights_stay_with_their_rows():
     from attnres.loss import linear_cross_entropy
     hidden, weight, targets = _case(30, 300, 64, BF16)
@@ -236,8 +297,10 @@ def test_linear_cross_entropy_strange_upstream_weights_stay_with_their_rows():
 
 
 @pytest.mark.parametrize("rows,vocabulary,width,ignored", [
-    (40000, 8200, 64, 0.0),      # two pieces of the vocabulary
-    (66000, 4999, 40, 0.2),      # two blocks of rows, two pieces, the last of them short
+    (40000, 8200, 64, 0.0),
+    (66000, 4999, 40, 0.2),      # two blocks of rows
+    (70000, 8300, 40, 0.2),      # and two pieces of the vocabulary, the last of them short
+    (66500, 8300, 512, 0.1),     # gradients in the forward, two pieces of the rows
 ])
 def test_linear_cross_entropy_in_pieces(rows, vocabulary, width, ignored):
     hidden, weight, targets = _case(rows, vocabulary, width, BF16, ignored=ignored, seed=7)
@@ -291,9 +354,10 @@ def test_linear_cross_entropy_no_rows():
 
 
 @pytest.mark.parametrize("needed", ["hidden", "weight"])
-def test_linear_cross_entropy_only_the_gradient_that_is_wanted(needed):
+@pytest.mark.parametrize("width", [72, 512])
+def test_linear_cross_entropy_only_the_gradient_that_is_wanted(needed, width):
     from attnres.loss import linear_cross_entropy
-    hidden, weight, targets = _case(150, 300, 72, BF16, seed=9)
+    hidden, weight, targets = _case(150, 300, width, BF16, seed=9)
     both = _check(hidden, weight, targets)
     hidden, weight = hidden.detach(), weight.detach()
     leaf = (hidden if needed == "hidden" else weight).requires_grad_()
@@ -327,9 +391,10 @@ def test_linear_cross_entropy_gradient_against_differences():
         assert abs(slope - along) < 2.0**-8 * size + 0.02, (slope, along)
 
 
-def test_linear_cross_entropy_compiles_and_captures():
+@pytest.mark.parametrize("width", [64, 576])
+def test_linear_cross_entropy_compiles_and_captures(width):
     from attnres.loss import linear_cross_entropy
-    hidden, weight, targets = _case(160, 300, 64, BF16, ignored=0.2, seed=11)
+    hidden, weight, targets = _case(160, 300, width, BF16, ignored=0.2, seed=11)
     leaves = [hidden.requires_grad_(), weight.requires_grad_()]
     for reduction in ("mean", "none"):
         call = lambda h, w, t: linear_cross_entropy(h, w, t, reduction=reduction)  # noqa: E731
@@ -350,7 +415,7 @@ def test_linear_cross_entropy_compiles_and_captures():
     with torch.cuda.graph(graph):
         loss = linear_cross_entropy(*static, ids)
         grads = torch.autograd.grad(loss, static)
-    other = _case(160, 300, 64, BF16, ignored=0.7, seed=12)   # another number of rows that count
+    other = _case(160, 300, width, BF16, ignored=0.7, seed=12)   # another number of rows that count
     with torch.no_grad():
         for dst, src in zip((*static, ids), other):
             dst.copy_(src)
@@ -382,17 +447,22 @@ def test_linear_cross_entropy_writes_only_its_outputs():
         sums, losses = take("sums", rows, FP32), take("losses", rows, FP32)
         loss, dh = take("loss", 1, FP32), take("dh", rows * width, BF16)
         dw = take("dw", vocabulary * width, BF16)
-        size = _native.loss_workspace_bytes(rows, vocabulary, width, False)
+        size = _native.loss_workspace_bytes(rows, vocabulary, width, _native.LOSS_FORWARD)
         space = take("space", size // 4, FP32)
         stream = torch.cuda.current_stream().cuda_stream
         common = (targets.data_ptr(), 1, rows, vocabulary, width, 0, -100, 1.0, 2)
         _native.loss_forward(hidden.data_ptr(), width, weight.data_ptr(), width, *common, kept, index,
-                             target, count, sums, losses, loss, space, size, stream)
-        size = _native.loss_workspace_bytes(rows, vocabulary, width, True)
+                             target, count, sums, losses, loss, None, None, space, size, stream)
+        size = _native.loss_workspace_bytes(rows, vocabulary, width, _native.LOSS_BACKWARD)
         space = take("space back", size // 4, FP32)
         one = torch.ones(1, device="cuda")
         _native.loss_backward(one.data_ptr(), 1, weight.data_ptr(), width, *common, kept, index, target,
                               count, sums, dh, dw, space, size, stream)
+        size = _native.loss_workspace_bytes(rows, vocabulary, width, _native.LOSS_FORWARD_GRADIENTS)
+        space = take("space gradients", size // 4, FP32)
+        dh, dw = take("dh early", rows * width, BF16), take("dw early", vocabulary * width, BF16)
+        _native.loss_forward(hidden.data_ptr(), width, weight.data_ptr(), width, *common, kept, index,
+                             target, count, None, losses, loss, dh, dw, space, size, stream)
         torch.cuda.synchronize()
         for name, whole in buffers.items():
             assert bool((whole[:pad] == -7).all()) and bool((whole[-pad:] == -7).all()), name
