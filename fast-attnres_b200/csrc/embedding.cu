@@ -40,26 +40,6 @@ int launch_embedding_forward(const EmbedParams& p, int lanes, dim3 grid, cudaStr
   return launched();
 }
 
-// A launch that may start before the kernel in front of it has ended (that kernel says when).
-template <typename... Parameters, typename... Arguments>
-int launch_beside(void (*kernel)(Parameters...), int64_t grid, int threads, bool beside,
-                  cudaStream_t stream, Arguments... arguments) {
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)grid);
-  config.blockDim = dim3((unsigned)threads);
-  config.stream = stream;
-  cudaLaunchAttribute early;
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &early;
-  config.numAttrs = beside ? 1 : 0;
-  if (cudaLaunchKernelEx(&config, kernel, Parameters(arguments)...) != cudaSuccess) {
-    cudaGetLastError();
-    return ATTNRES_B200_ERR_CUDA;
-  }
-  return ATTNRES_B200_OK;
-}
-
 template <bool VECTOR, bool WIDE>
 int launch_embedding_backward(const EmbedParams& p, int sms, cudaStream_t cs) {
   static SmemGrant grant;
@@ -76,8 +56,8 @@ int launch_embedding_backward(const EmbedParams& p, int sms, cudaStream_t cs) {
   }
   if (p.dpositions != nullptr)
     position_ctas = (p.T * ((p.D + 7) / 8) + kEarlyThreads - 1) / kEarlyThreads;
-  if (int st = launch_beside(embedding_early_kernel<VECTOR, WIDE>, fill_ctas + position_ctas,
-                             kEarlyThreads, p.dtable != nullptr, cs, p, type_bytes(p.table_type),
+  if (int st = launch_behind(embedding_early_kernel<VECTOR, WIDE>, fill_ctas + position_ctas,
+                             kEarlyThreads, 0, p.dtable != nullptr, cs, p, type_bytes(p.table_type),
                              (int)fill_ctas))
     return st;
   if (p.dtable == nullptr) return ATTNRES_B200_OK;
@@ -91,8 +71,8 @@ int launch_embedding_backward(const EmbedParams& p, int sms, cudaStream_t cs) {
   if (tiles == 1) return ATTNRES_B200_OK;
   constexpr int warps = kEmbedThreads / 32;
   const int64_t joins = (units + warps - 1) / warps;
-  return launch_beside(embedding_join_kernel<VECTOR>, joins < 2 * sms ? joins : 2 * sms,
-                       kEmbedThreads, true, cs, p, lanes, blocks, tiles);
+  return launch_behind(embedding_join_kernel<VECTOR>, joins < 2 * sms ? joins : 2 * sms,
+                       kEmbedThreads, 0, true, cs, p, lanes, blocks, tiles);
 }
 
 int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }

@@ -162,7 +162,7 @@ constexpr uint32_t kSortSmem = (kSortWarps + 2) * kSortDigits * 4 + 64;
 __global__ void __cluster_dims__(kSortCluster, 1, 1) __launch_bounds__(kSortThreads, 1)
 embedding_sort_kernel(const EmbedParams p) {
   // The kernel beside this one may start at once; it waits for this one before it ends.
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  start_next_kernel();
   extern __shared__ uint32_t smem[];
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.runs = 0;
   namespace cg = cooperative_groups;
@@ -316,7 +316,7 @@ embedding_early_kernel(const EmbedParams p, int element_bytes, int fill_ctas) {
     }
   }
   // What follows in the stream waits for this kernel, and through this also for the sort.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous_kernel();
 }
 
 // ------------------------------------------------------------------------------ gradient, step 2
@@ -326,7 +326,7 @@ constexpr int kJoinBatch = 8;  // pieces in flight per lane
 template <bool VECTOR, bool WIDE>
 __global__ void __launch_bounds__(kEmbedThreads)
 embedding_sum_kernel(const EmbedParams p, int lanes, int blocks, int64_t tiles) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining waits for the end
+  start_next_kernel();  // the joining waits for the end
   constexpr int E = gradient_columns<VECTOR>();
   constexpr int kSumBatch = VECTOR ? 8 : 16;  // rows in flight per lane
   const int lane = threadIdx.x % lanes;
@@ -403,7 +403,7 @@ embedding_sum_kernel(const EmbedParams p, int lanes, int blocks, int64_t tiles) 
 template <bool VECTOR>
 __global__ void __launch_bounds__(kEmbedThreads)
 embedding_join_kernel(const EmbedParams p, int lanes, int blocks, int64_t tiles) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous_kernel();
   constexpr int E = gradient_columns<VECTOR>();
   const int lane = threadIdx.x & 31;
   const uint2* pairs = p.pairs[(p.passes - 1) & 1];

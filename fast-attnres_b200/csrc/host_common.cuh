@@ -49,4 +49,34 @@ inline bool aligned_type(const void* p, int32_t type) {
   return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(type_bytes(type) - 1)) == 0;
 }
 
+// A launch that may begin before the kernel in front of it has ended: once all of that kernel's CTAs
+// have called start_next_kernel() or are done.  The launched kernel calls wait_for_previous_kernel()
+// before it touches anything the kernels in front of it read or write.
+template <typename... Parameters, typename... Arguments>
+int launch_behind(void (*kernel)(Parameters...), int64_t grid, int threads, uint32_t smem, bool behind,
+                  cudaStream_t stream, const Arguments&... arguments) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)grid);
+  config.blockDim = dim3((unsigned)threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = behind ? 1 : 0;
+  if (cudaLaunchKernelEx(&config, kernel, Parameters(arguments)...) != cudaSuccess) {
+    cudaGetLastError();
+    return ATTNRES_B200_ERR_CUDA;
+  }
+  return ATTNRES_B200_OK;
+}
+
+__device__ __forceinline__ void start_next_kernel() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_previous_kernel() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 }  // namespace attnres_b200

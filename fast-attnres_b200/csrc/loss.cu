@@ -104,7 +104,7 @@ int64_t tiles_of(int64_t rows, int64_t columns, bool pair) {
 
 // Pairs of CTAs load a third less for the same products; single CTAs make twice as many, smaller
 // tiles, which is what counts when there are few.
-bool use_pairs(int64_t tiles_of_pairs) { return tiles_of_pairs >= 148; }
+bool use_pairs(int64_t tiles_of_pairs) { return tiles_of_pairs >= 296; }
 
 LossPlan plan_loss(int64_t N, int32_t V, int32_t D) {
   LossPlan plan;
@@ -165,13 +165,15 @@ int launch_product(const CUtensorMap (&maps)[3], const ProductParams& p, int64_t
   config.blockDim = dim3(kProductThreads);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  cudaLaunchAttribute cluster;
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = 2;
-  cluster.val.clusterDim.y = 1;
-  cluster.val.clusterDim.z = 1;
-  config.attrs = &cluster;
-  config.numAttrs = PAIR ? 1 : 0;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = 2;
+  attributes[1].val.clusterDim.y = 1;
+  attributes[1].val.clusterDim.z = 1;
+  config.attrs = attributes;
+  config.numAttrs = PAIR ? 2 : 1;
   if (cudaLaunchKernelEx(&config, loss_product_kernel<PASS, T, PAIR>, maps[0], maps[1], maps[2],
                          p) != cudaSuccess) {
     cudaGetLastError();
@@ -194,14 +196,16 @@ int launch_product_type(int32_t type, const CUtensorMap (&maps)[3], const Produc
 
 // The weight as the TMA can read it: in place, or copied into rows of a multiple of eight.
 int lay_out_weight(const void** weight, int64_t* row_stride, int32_t V, int32_t D, void* copy,
-                   int sms, cudaStream_t stream) {
+                   bool behind, int sms, cudaStream_t stream) {
   if (!needs_padding(*weight, *row_stride, V, D)) return ATTNRES_B200_OK;
-  loss_pad_kernel<<<sms * 8, 256, 0, stream>>>(static_cast<unsigned short*>(copy),
-                                               static_cast<const unsigned short*>(*weight),
-                                               *row_stride, V, D, padded_width(D));
+  if (int st = launch_behind(loss_pad_kernel, sms * 8, 256, 0, behind, stream,
+                             static_cast<unsigned short*>(copy),
+                             static_cast<const unsigned short*>(*weight), *row_stride, (int64_t)V, D,
+                             padded_width(D)))
+    return st;
   *weight = copy;
   *row_stride = padded_width(D);
-  return launched();
+  return ATTNRES_B200_OK;
 }
 
 }  // namespace
@@ -292,7 +296,7 @@ extern "C" int attnres_b200_loss_forward(
   else
     loss_gather_kernel<false><<<gather_grid, kGatherThreads, 0, cs>>>(g);
   if (int st = launched()) return st;
-  if (int st = lay_out_weight(&weight, &weight_row_stride, V, D, space, sms, cs)) return st;
+  if (int st = lay_out_weight(&weight, &weight_row_stride, V, D, space, true, sms, cs)) return st;
 
   CUtensorMap maps[3];
   if (int st = make_map(&maps[0], kept, type, N, D, Dp, 64)) return st;
@@ -327,10 +331,11 @@ extern "C" int attnres_b200_loss_forward(
       if (int st = make_map(&use[0], codes, type, p.row_limit, V, stride, 64)) return st;
       const auto logits = [&](bool pair) { return tiles_of(p.row_limit, V, pair); };
       if (int st = launch_product_type<kCodes>(type, form, p, logits, sms, cs)) return st;
-      loss_probs_kernel<<<p.row_limit < 8 * sms ? p.row_limit : 8 * sms, kJoinThreads, 0, cs>>>(
-          partials, pairs, count, p.first_row, p.row_limit, target_logit, kept_target, kept_index,
-          losses, codes, stride, V);
-      if (int st = launched()) return st;
+      if (int st = launch_behind(loss_probs_kernel, p.row_limit < 8 * sms ? p.row_limit : 8 * sms,
+                                 kJoinThreads, 0, true, cs, partials, pairs, count, p.first_row,
+                                 p.row_limit, target_logit, kept_target, kept_index, losses, codes,
+                                 stride, V))
+        return st;
       p.weight_out = dweight != nullptr && pieces.pieces > 1 ? weight_parts + piece * V * D : nullptr;
       const auto both = [&](bool pair) {
         return (dhidden ? tiles_of(p.row_limit, D, pair) : 0) + (dweight ? tiles_of(V, D, pair) : 0);
@@ -338,11 +343,11 @@ extern "C" int attnres_b200_loss_forward(
       if (int st = launch_product_type<kGradients>(type, use, p, both, sms, cs)) return st;
     }
     if (p.weight_out != nullptr) {
-      loss_slices_kernel<<<8 * sms, 256, 0, cs>>>(weight_parts, (int)pieces.pieces, nullptr, nullptr,
-                                                  gradient_scale, scale, V, D,
-                                                  static_cast<__nv_bfloat16*>(dweight),
-                                                  p.vector_dweight);
-      if (int st = launched()) return st;
+      if (int st = launch_behind(loss_slices_kernel<__nv_bfloat16>, 8 * sms, 256, 0, true, cs,
+                                 weight_parts, (int)pieces.pieces, nullptr, nullptr, gradient_scale,
+                                 scale, (int64_t)V, D, static_cast<__nv_bfloat16*>(dweight),
+                                 p.vector_dweight))
+        return st;
     }
   }
   for (int64_t row = 0; row < N && !gradients; row += plan.stats_rows) {
@@ -350,13 +355,14 @@ extern "C" int attnres_b200_loss_forward(
     p.row_limit = (int32_t)(N - row < plan.stats_rows ? N - row : plan.stats_rows);
     const auto tiles = [&](bool pair) { return tiles_of(p.row_limit, V, pair); };
     if (int st = launch_product_type<kStats>(type, maps, p, tiles, sms, cs)) return st;
-    loss_join_kernel<<<p.row_limit < 8 * sms ? p.row_limit : 8 * sms, kJoinThreads, 0, cs>>>(
-        partials, pairs, count, p.first_row, p.row_limit, target_logit, kept_index, lse2, losses);
-    if (int st = launched()) return st;
+    if (int st = launch_behind(loss_join_kernel, p.row_limit < 8 * sms ? p.row_limit : 8 * sms,
+                               kJoinThreads, 0, true, cs, partials, pairs, count, p.first_row,
+                               p.row_limit, target_logit, kept_index, lse2, losses))
+      return st;
   }
   if (reduction == ATTNRES_B200_LOSS_NONE) return ATTNRES_B200_OK;
-  loss_reduce_kernel<<<1, 1024, 0, cs>>>(losses, N, count, reduction == ATTNRES_B200_LOSS_MEAN, loss);
-  return launched();
+  return launch_behind(loss_reduce_kernel, 1, 1024, 0, true, cs, losses, N, count,
+                       (int)(reduction == ATTNRES_B200_LOSS_MEAN), loss);
 }
 
 extern "C" int attnres_b200_loss_backward(
@@ -390,14 +396,16 @@ extern "C" int attnres_b200_loss_backward(
       reinterpret_cast<float*>(space + plan.padded_weight + plan.probs + plan.slices_out);
   float* weight_of = gradient_scale + 1;
 
-  if (int st = lay_out_weight(&weight, &weight_row_stride, V, D, space, sms, cs)) return st;
+  const bool padded = needs_padding(weight, weight_row_stride, V, D);
+  if (int st = lay_out_weight(&weight, &weight_row_stride, V, D, space, false, sms, cs)) return st;
   const int64_t zero_ctas = (N + 31) / 32;
-  loss_weights_kernel<<<1 + (int)(zero_ctas < 2 * sms ? zero_ctas : 2 * sms), 1024, 0, cs>>>(
-      upstream, upstream_stride, reduction == ATTNRES_B200_LOSS_NONE,
-      reduction == ATTNRES_B200_LOSS_MEAN, count, kept_index,
-      type == ATTNRES_B200_FP16 ? kHalfLift : 1.f, weight_of, gradient_scale, targets, targets_64,
-      ignored, N, static_cast<unsigned short*>(dhidden), D);
-  if (int st = launched()) return st;
+  if (int st = launch_behind(loss_weights_kernel, 1 + (zero_ctas < 2 * sms ? zero_ctas : 2 * sms), 1024,
+                             0, padded, cs, upstream, upstream_stride,
+                             (int)(reduction == ATTNRES_B200_LOSS_NONE),
+                             (int)(reduction == ATTNRES_B200_LOSS_MEAN), count, kept_index,
+                             type == ATTNRES_B200_FP16 ? kHalfLift : 1.f, weight_of, gradient_scale,
+                             targets, targets_64, ignored, N, static_cast<unsigned short*>(dhidden), D))
+    return st;
 
   CUtensorMap map_h, map_w;
   if (int st = make_map(&map_h, kept, type, N, D, Dp, 64)) return st;
@@ -440,14 +448,12 @@ extern "C" int attnres_b200_loss_backward(
   const int64_t ctas = (N + 7) / 8;
   const unsigned grid = (unsigned)(ctas < 8 * sms ? ctas : 8 * sms);
   if (type == ATTNRES_B200_BF16)
-    loss_slices_kernel<<<grid, 256, 0, cs>>>(slices_out, p.first_slice, count, kept_index,
-                                             gradient_scale, scale, N, D,
-                                             static_cast<__nv_bfloat16*>(dhidden), p.vector_dhidden);
-  else
-    loss_slices_kernel<<<grid, 256, 0, cs>>>(slices_out, p.first_slice, count, kept_index,
-                                             gradient_scale, scale, N, D,
-                                             static_cast<__half*>(dhidden), p.vector_dhidden);
-  return launched();
+    return launch_behind(loss_slices_kernel<__nv_bfloat16>, grid, 256, 0, true, cs, slices_out,
+                         p.first_slice, count, kept_index, gradient_scale, scale, N, D,
+                         static_cast<__nv_bfloat16*>(dhidden), p.vector_dhidden);
+  return launch_behind(loss_slices_kernel<__half>, grid, 256, 0, true, cs, slices_out, p.first_slice,
+                       count, kept_index, gradient_scale, scale, N, D, static_cast<__half*>(dhidden),
+                       p.vector_dhidden);
 }
 
 extern "C" int32_t attnres_b200_loss_gradients_in_forward(int32_t D, int32_t type, int32_t reduction) {

@@ -63,11 +63,11 @@ template <bool VECTOR>
 __device__ __forceinline__ void copy_row(unsigned short* dst, const unsigned short* src, int D,
                                          int Dp, int lane) {
   if (VECTOR && src != nullptr) {
-#pragma unroll 4
+#pragma unroll 8
     for (int c = lane; c < Dp / 8; c += 32)
       reinterpret_cast<uint4*>(dst)[c] = __ldg(reinterpret_cast<const uint4*>(src) + c);
   } else {
-#pragma unroll 4
+#pragma unroll 16
     for (int i = lane; i < Dp; i += 32)
       dst[i] = (src != nullptr && i < D) ? __ldg(src + i) : (unsigned short)0;
   }
@@ -77,6 +77,8 @@ constexpr int kGatherThreads = 1024;
 
 template <bool VECTOR>
 __global__ void __launch_bounds__(kGatherThreads) loss_gather_kernel(const GatherParams p) {
+  start_next_kernel();
+  wait_for_previous_kernel();
   __shared__ int warp_counts[kGatherThreads / 32];
   __shared__ int places[kGatherThreads];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -145,6 +147,8 @@ __global__ void __launch_bounds__(kGatherThreads) loss_gather_kernel(const Gathe
 __global__ void __launch_bounds__(256)
 loss_pad_kernel(unsigned short* dst, const unsigned short* src, int64_t row_stride, int64_t rows,
                 int D, int Dp) {
+  start_next_kernel();
+  wait_for_previous_kernel();
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8)
     copy_row<false>(dst + r * Dp, src + r * row_stride, D, Dp, threadIdx.x & 31);
 }
@@ -173,6 +177,10 @@ constexpr uint32_t product_smem(bool pair) {
 // FP16 keeps P times 2^15: probabilities of a large vocabulary would be subnormal.
 constexpr float kHalfLift = 32768.f;
 constexpr float kCodeSteps = 2048.f;  // of a code, to a power of two
+// Steps of K (1024 features) after which a tile of logits goes to registers and is added there.  The
+// tensor cores truncate as they add, which shrinks a logit by about D 10^-9 of itself: at 4096
+// features the loss was off by 1.8e-6, in segments of 1024 by MEASURE.
+constexpr int kSegmentSteps = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -294,12 +302,14 @@ template <int PASS, bool PAIR>
 struct TileOrder {
   static constexpr int kRows = tile_rows(PAIR);
   int tiles_m, tiles_n, steps;     // kGradients: of dH
+  int width = kTileN;              // kGradients: columns of a tile, D spread evenly over the tiles
   int weight_m, weight_steps, slice_steps;
   int hidden_tiles, total;
 
   __device__ TileOrder(const ProductParams& p, int rows) {
     if constexpr (PASS == kGradients) {
       tiles_n = (p.D + kTileN - 1) / kTileN;
+      width = ((p.D + tiles_n - 1) / tiles_n + 31) / 32 * 32;
       tiles_m = p.dhidden != nullptr ? (rows + kRows - 1) / kRows : 0;
       steps = (p.vn + kTileK - 1) / kTileK;
       slice_steps = (steps + p.slices - 1) / p.slices;
@@ -335,7 +345,7 @@ struct TileOrder {
       }
       const int row = rest / tiles_n;
       t.m = row * kRows;
-      t.n = (rest - row * tiles_n) * kTileN;
+      t.n = (rest - row * tiles_n) * width;
     } else {
       constexpr int kGroup = 2048 / kRows;
       const int group = index / (kGroup * tiles_n), rest = index - group * kGroup * tiles_n;
@@ -369,9 +379,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
   const int worker = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
   const int workers = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
   const uint32_t stages = (smem_addr(product_memory) + 1023u) & ~1023u;
-  // Kept rows of this launch, counted from first_row on.
-  const int kept = min(max(*p.count - p.first_row, 0), p.row_limit);
-  const TileOrder<PASS, PAIR> order(p, kept);
+  start_next_kernel();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -394,6 +402,11 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
   if constexpr (PAIR) cluster_barrier();  // the other CTA's barriers exist
   tcgen05_fence_after();
   const uint32_t tmem = tmem_slot;
+  // All of this ran beside the end of the kernel in front; its results are used from here on.
+  wait_for_previous_kernel();
+  // Kept rows of this launch, counted from first_row on.
+  const int kept = min(max(*p.count - p.first_row, 0), p.row_limit);
+  const TileOrder<PASS, PAIR> order(p, kept);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -406,8 +419,9 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
         const bool a_mn = PASS == kGradients && t.weight;
         const CUtensorMap* map_b = PASS == kGradients && t.weight ? &map_2 : &map_1;
         const int a0 = t.m + rank * kCtaRows + (PASS != kGradients ? p.first_row : 0);
-        const int b0 = t.n + rank * (kTileN / 2) + (PASS == kGradients ? 0 : p.v0);
+        const int b0 = t.n + rank * (order.width / 2) + (PASS == kGradients ? 0 : p.v0);
         const int bk = PASS != kGradients ? 0 : t.weight ? p.first_row : p.v0;
+        const int boxes = PASS != kGradients ? kBoxesB : (order.width / (PAIR ? 2 : 1) + 63) / 64;
         for (int k = t.k_first; k < t.k_first + t.k_steps; ++k) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, &abort_flag)) {
             alive = false;
@@ -415,17 +429,19 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
           }
           uint32_t bar = smem_addr(&full[stage]);
           if constexpr (PAIR) bar = cluster_address(bar, 0);
-          if (rank == 0) mbar_expect_tx(&full[stage], kStageBytes * (PAIR ? 2 : 1));
+          if (rank == 0) mbar_expect_tx(&full[stage], (2 + boxes) * kBoxBytes * (PAIR ? 2 : 1));
           const uint32_t a = stages + stage * kStageBytes, b = a + 2 * kBoxBytes;
 #pragma unroll
           for (int j = 0; j < 2; ++j)
             tensor_load_2d<PAIR>(a + j * kBoxBytes, &map_0, a_mn ? a0 + j * 64 : k * kTileK,
                                  a_mn ? k * kTileK : a0 + j * 64, bar);
 #pragma unroll
-          for (int j = 0; j < kBoxesB; ++j)
-            tensor_load_2d<PAIR>(b + j * kBoxBytes, map_b,
-                                 PASS == kGradients ? b0 + j * 64 : k * kTileK,
-                                 PASS == kGradients ? bk + k * kTileK : b0 + j * 64, bar);
+          for (int j = 0; j < kBoxesB; ++j) {
+            if (PASS != kGradients || j < boxes)
+              tensor_load_2d<PAIR>(b + j * kBoxBytes, map_b,
+                                   PASS == kGradients ? b0 + j * 64 : k * kTileK,
+                                   PASS == kGradients ? bk + k * kTileK : b0 + j * 64, bar);
+          }
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
@@ -440,38 +456,43 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
       bool alive = true;
       for (int i = worker; i < order.total && alive; i += workers) {
         const Tile t = order.at(i);
-        if (!mbar_wait(&taken[buffer], buffer_phase ^ 1u, &abort_flag)) break;
-        tcgen05_fence_after();
-        const uint32_t d = tmem + buffer * kTileN;
         // 16 elements of K: 32 bytes along a K-major row, two 1 KB groups of MN-major rows.
         const bool a_mn = PASS == kGradients && t.weight;
-        const uint32_t instruction = a_mn
-            ? mma_instruction(kBf16, true, PASS == kGradients, kRows, kTileN)
-            : mma_instruction(kBf16, false, PASS == kGradients, kRows, kTileN);
+        const uint32_t instruction = mma_instruction(kBf16, a_mn, PASS == kGradients, kRows, order.width);
         const uint32_t step_a = (a_mn ? 2048 : 32) >> 4;
         constexpr uint32_t step_b = (PASS == kGradients ? 2048 : 32) >> 4;
-        for (int k = 0; k < t.k_steps; ++k) {
-          if (!mbar_wait(&full[stage], phase, &abort_flag)) {
+        int k = 0;
+        do {
+          const int last = PASS == kGradients ? t.k_steps : min(t.k_steps, k + kSegmentSteps);
+          if (!mbar_wait(&taken[buffer], buffer_phase ^ 1u, &abort_flag)) {
             alive = false;
             break;
           }
           tcgen05_fence_after();
-          const uint32_t a = stages + stage * kStageBytes, b = a + 2 * kBoxBytes;
-          const uint64_t da = operand_descriptor(a), db = operand_descriptor(b);
+          const uint32_t d = tmem + buffer * kTileN;
+          for (int first = k; k < last; ++k) {
+            if (!mbar_wait(&full[stage], phase, &abort_flag)) {
+              alive = false;
+              break;
+            }
+            tcgen05_fence_after();
+            const uint32_t a = stages + stage * kStageBytes, b = a + 2 * kBoxBytes;
+            const uint64_t da = operand_descriptor(a), db = operand_descriptor(b);
 #pragma unroll
-          for (int kk = 0; kk < kTileK / 16; ++kk)
-            tcgen05_mma_f16<PAIR>(d, da + kk * step_a, db + kk * step_b, instruction,
-                                  k > 0 || kk > 0);
-          tcgen05_commit<PAIR>(&empty[stage]);
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1u;
+            for (int kk = 0; kk < kTileK / 16; ++kk)
+              tcgen05_mma_f16<PAIR>(d, da + kk * step_a, db + kk * step_b, instruction,
+                                    k > first || kk > 0);
+            tcgen05_commit<PAIR>(&empty[stage]);
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
-        }
-        if (!alive) break;
-        tcgen05_commit<PAIR>(&done[buffer]);
-        buffer ^= 1;
-        if (buffer == 0) buffer_phase ^= 1u;
+          if (!alive) break;
+          tcgen05_commit<PAIR>(&done[buffer]);
+          buffer ^= 1;
+          if (buffer == 0) buffer_phase ^= 1u;
+        } while (k < t.k_steps);
       }
     }
   } else {
@@ -491,8 +512,10 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
     for (int i = worker; i < order.total; i += workers) {
       const Tile t = order.at(i);
       const int first_row = t.m + rank * kCtaRows + quad * 32, row = first_row + lane;
-      const int column = t.n + half * (kTileN / 2);
-      // What the row needs is fetched while the products run.
+      const int column = t.n + half * (order.width / 2);
+      // What the row needs is fetched while the products run.  Rows beyond the kept ones are zeros
+      // up to a multiple of 128, which gives them P = 0 (the sums over rows reach up to the next
+      // multiple of 64).
       int target = -1;
       float lse2 = 0.f, weight_of = 0.f;
       bool live = true;
@@ -509,100 +532,112 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
       }
       if (!mbar_wait(&done[buffer], buffer_phase, &abort_flag)) break;
       tcgen05_fence_after();
-      const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + buffer * kTileN + half * (kTileN / 2);
-      if constexpr (PASS == kStats || PASS == kCodes) {
-        // The half tile's maximum first: sums and codes count from it.
-        float top = -INFINITY, sum = 0.f;
-#pragma unroll 1
-        for (int c = 0; c < kTileN / 2 && column + c < p.vn; c += 32) {
-          uint32_t r[32];
-          tmem_load_32(src + c, r);
-          const int valid = p.vn - column - c;
+      uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + buffer * kTileN + half * (order.width / 2);
+      auto release = [&] {
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR) mbar_arrive_cluster(taken_bar[buffer]);
+          else mbar_arrive(&taken[buffer]);
+        }
+        buffer ^= 1;
+        if (buffer == 0) buffer_phase ^= 1u;
+      };
+      const int columns = min(order.width / 2, p.D - column);  // of this half tile of a gradient
+      if constexpr (PASS != kGradients) {
+        // The row's 128 logits of the half tile, segment by segment, before anything is done with
+        // them: the next tile's products can go on.
+        float z[kTileN / 2];
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            top = fmaxf(top, e < valid ? __uint_as_float(r[e]) * to_log2 : -INFINITY);
+        for (int c = 0; c < kTileN / 2; c += 32)
+          tmem_load_32(src + c, *reinterpret_cast<uint32_t(*)[32]>(z + c));
+        release();
+        bool alive = true;
+        for (int k = kSegmentSteps; k < t.k_steps; k += kSegmentSteps) {
+          if (!mbar_wait(&done[buffer], buffer_phase, &abort_flag)) {
+            alive = false;
+            break;
+          }
+          tcgen05_fence_after();
+          src = tmem + ((uint32_t)(quad * 32) << 16) + buffer * kTileN + half * (kTileN / 2);
+#pragma unroll
+          for (int c = 0; c < kTileN / 2; c += 16) {
+            uint32_t r[16];
+            tmem_load_16(src + c, r);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) z[c + e] += __uint_as_float(r[e]);
+          }
+          release();
+        }
+        if (!alive) break;
+        const int valid = p.vn - column, at = target - column;
+        const bool rows_exist = first_row < p.row_limit;
+        float top = -INFINITY, sums[2] = {0.f, 0.f};
+        if constexpr (PASS == kStats || PASS == kCodes) {
+          // The half tile's maximum first: sums and codes count from it.
+#pragma unroll
+          for (int e = 0; e < kTileN / 2; ++e) z[e] *= to_log2;
+          if (valid < kTileN / 2) {  // the last tile: ids beyond the vocabulary
+#pragma unroll
+            for (int e = 0; e < kTileN / 2; ++e) z[e] = e < valid ? z[e] : -INFINITY;
+          }
+#pragma unroll
+          for (int e = 0; e < kTileN / 2; ++e) top = fmaxf(top, z[e]);
+          if (at >= 0 && at < kTileN / 2) {
+            float y = z[0];
+#pragma unroll
+            for (int e = 1; e < kTileN / 2; ++e) y = at == e ? z[e] : y;
+            p.target_logit[p.first_row + row] = y;
+          }
         }
         const float pivot = top == -INFINITY ? 0.f : top;
-        const bool rows_exist = first_row < p.row_limit;
-#pragma unroll 1
-        for (int c = 0; c < kTileN / 2 && column + c < p.vn; c += 64) {
-          if constexpr (PASS == kCodes) {
-            if (lane == 0) tensor_store_wait_read();
-            __syncwarp();
-          }
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t r[32];
-            tmem_load_32(src + c + h * 32, r);
-            const int valid = p.vn - column - c - h * 32, at = target - column - c - h * 32;
-            if (at >= 0 && at < 32) {
-              float z = __uint_as_float(r[0]);
-#pragma unroll
-              for (int e = 1; e < 32; ++e) z = at == e ? __uint_as_float(r[e]) : z;
-              p.target_logit[p.first_row + row] = z * to_log2;
+        for (int c = 0; c < kTileN / 2; c += 64) {
+          if (column + c < p.vn) {
+            if constexpr (PASS != kStats) {
+              if (lane == 0) tensor_store_wait_read();
+              __syncwarp();
             }
-            float part = 0.f;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float down = fmaf(__uint_as_float(r[e]), to_log2, -pivot);  // at most zero
-              part += e < valid ? exp2_approx(down) : 0.f;
-              if constexpr (PASS == kCodes) {
-                // Adding 2^23 leaves the rounded integer in the low bits.
-                const float code = fminf(fmaf(down, -kCodeSteps, 8388608.f), 8388608.f + 65535.f);
-                r[e] = live ? __float_as_uint(code) : 0u;
+            for (int h = 0; h < 64; h += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const int e = c + h + 2 * q;
+                if constexpr (PASS == kProbs) {
+                  const float p0 = exp2_approx(fmaf(z[e], to_log2, -lse2));
+                  const float p1 = exp2_approx(fmaf(z[e + 1], to_log2, -lse2));
+                  const float v0 = weight_of * (at == e ? p0 - 1.f : p0);
+                  const float v1 = weight_of * (at == e + 1 ? p1 - 1.f : p1);
+                  w[q] = pack2<T>(v0, v1);
+                } else {
+                  const float down0 = z[e] - pivot, down1 = z[e + 1] - pivot;  // at most zero
+                  sums[0] += exp2_approx(down0);
+                  sums[1] += exp2_approx(down1);
+                  if constexpr (PASS == kCodes) {
+                    // Adding 2^23 leaves the rounded integer in the low bits.
+                    const float most = 8388608.f + 65535.f;
+                    const float code0 = fminf(fmaf(down0, -kCodeSteps, 8388608.f), most);
+                    const float code1 = fminf(fmaf(down1, -kCodeSteps, 8388608.f), most);
+                    w[q] = __byte_perm(__float_as_uint(code0), __float_as_uint(code1), 0x5410);
+                  }
+                }
               }
+              if constexpr (PASS != kStats)
+                store_shared16(block_slot(staging, lane, h / 8), w[0], w[1], w[2], w[3]);
             }
-            sum += part;
-            if constexpr (PASS == kCodes) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                store_shared16(block_slot(staging, lane, h * 4 + q),
-                               __byte_perm(r[8 * q], r[8 * q + 1], 0x5410),
-                               __byte_perm(r[8 * q + 2], r[8 * q + 3], 0x5410),
-                               __byte_perm(r[8 * q + 4], r[8 * q + 5], 0x5410),
-                               __byte_perm(r[8 * q + 6], r[8 * q + 7], 0x5410));
+            if constexpr (PASS != kStats) {
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0 && rows_exist) tensor_store_2d(&map_2, column + c, first_row, staging);
             }
-          }
-          if constexpr (PASS == kCodes) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0 && rows_exist) tensor_store_2d(&map_2, column + c, first_row, staging);
           }
         }
-        if (live)
-          p.partials[(int64_t)row * (2 * order.tiles_n) + 2 * (t.n / kTileN) + half] =
-              make_float2(top, sum);
-      } else if constexpr (PASS == kProbs) {
-        const bool rows_exist = first_row < p.N;
-#pragma unroll 1
-        for (int c = 0; c < kTileN / 2 && column + c < p.vn; c += 64) {
-          if (lane == 0) tensor_store_wait_read();
-          __syncwarp();
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t r[32];
-            tmem_load_32(src + c + h * 32, r);
-            const int at = target - column - c - h * 32;
-            float v[32];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float prob = exp2_approx(fmaf(__uint_as_float(r[e]), to_log2, -lse2));
-              v[e] = weight_of * (at == e ? prob - 1.f : prob);
-            }
-            if (!live) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = 0.f;
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              store_shared16(block_slot(staging, lane, h * 4 + q), pack2<T>(v[8 * q], v[8 * q + 1]),
-                             pack2<T>(v[8 * q + 2], v[8 * q + 3]),
-                             pack2<T>(v[8 * q + 4], v[8 * q + 5]),
-                             pack2<T>(v[8 * q + 6], v[8 * q + 7]));
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0 && rows_exist) tensor_store_2d(&map_2, column + c, first_row, staging);
+        if constexpr (PASS == kStats || PASS == kCodes) {
+          // (a half tile beyond the vocabulary is all -inf: it adds nothing)
+          if (live)
+            p.partials[(int64_t)row * (2 * order.tiles_n) + 2 * (t.n / kTileN) + half] =
+                make_float2(top, sums[0] + sums[1]);
         }
       } else if ((t.weight ? p.weight_out : p.slices_out) != nullptr) {
         // A part of the sum: FP32, added to the others by loss_slices_kernel.
@@ -614,7 +649,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
         }
         float* parts = t.weight ? p.weight_out : p.slices_out;
 #pragma unroll 1
-        for (int c = 0; c < kTileN / 2 && column + c < p.D; c += 32) {
+        for (int c = 0; c < columns; c += 32) {
           uint32_t r[32];
           tmem_load_32(src + c, r);
 #pragma unroll
@@ -625,7 +660,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
             else
               store_shared16(block_slot(staging, lane, q), 0u, 0u, 0u, 0u);
           }
-          write_block<float>(staging, parts + c, place, p.D - column - c, p.D % 4 == 0, lane);
+          write_block<float>(staging, parts + c, place, columns - c, p.D % 4 == 0, lane);
         }
       } else {
         int64_t place = -1;
@@ -637,7 +672,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
         T* out = static_cast<T*>(t.weight ? p.dweight : p.dhidden);
         const bool vector = t.weight ? p.vector_dweight : p.vector_dhidden;
 #pragma unroll 1
-        for (int c = 0; c < kTileN / 2 && column + c < p.D; c += 64) {
+        for (int c = 0; c < columns; c += 64) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t r[32];
@@ -653,17 +688,10 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
                              pack2<T>(v[8 * q + 4], v[8 * q + 5]),
                              pack2<T>(v[8 * q + 6], v[8 * q + 7]));
           }
-          write_block<T>(staging, out + c, place, p.D - column - c, vector, lane);
+          write_block<T>(staging, out + c, place, columns - c, vector, lane);
         }
       }
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (PAIR) mbar_arrive_cluster(taken_bar[buffer]);
-        else mbar_arrive(&taken[buffer]);
-      }
-      buffer ^= 1;
-      if (buffer == 0) buffer_phase ^= 1u;
+      if constexpr (PASS == kGradients) release();
     }
     if ((PASS == kProbs || PASS == kCodes) && lane == 0) tensor_store_wait_read();
   }
@@ -690,6 +718,8 @@ __global__ void __launch_bounds__(256)
 loss_slices_kernel(const float* __restrict__ slices, int count, const int32_t* kept_rows,
                    const int32_t* __restrict__ kept_index, const float* gradient_scale, float scale,
                    int64_t N, int D, T* out, int vector) {
+  start_next_kernel();
+  wait_for_previous_kernel();
   const float out_scale = scale * *gradient_scale * (__is_same(T, __half) ? 1.f / kHalfLift : 1.f);
   const int lane = threadIdx.x & 31;
   const int64_t kept = kept_index != nullptr ? *kept_rows : N;
@@ -776,6 +806,8 @@ loss_join_kernel(const float2* __restrict__ partials, int pairs, const int32_t* 
                  int row_limit, const float* __restrict__ target_logit,
                  const int32_t* __restrict__ kept_index, float* __restrict__ lse2,
                  float* __restrict__ losses) {
+  start_next_kernel();
+  wait_for_previous_kernel();
   const int rows = min(max(*count - first_row, 0), row_limit);
   for (int row = blockIdx.x; row < rows; row += gridDim.x) {
     const float at_target = target_logit[first_row + row];
@@ -793,6 +825,8 @@ loss_probs_kernel(const float2* __restrict__ partials, int pairs, const int32_t*
                   int row_limit, const float* __restrict__ target_logit,
                   const int32_t* __restrict__ kept_target, const int32_t* __restrict__ kept_index,
                   float* __restrict__ losses, unsigned short* codes, int64_t stride, int V) {
+  start_next_kernel();
+  wait_for_previous_kernel();
   const int tid = threadIdx.x, rows = min(max(*count - first_row, 0), row_limit);
   for (int row = blockIdx.x; row < rows; row += gridDim.x) {
     const float2* mine = partials + (int64_t)row * pairs;
@@ -829,6 +863,8 @@ loss_probs_kernel(const float2* __restrict__ partials, int pairs, const int32_t*
 __global__ void __launch_bounds__(1024)
 loss_reduce_kernel(const float* __restrict__ losses, int64_t N, const int32_t* count, int mean,
                    float* out) {
+  start_next_kernel();
+  wait_for_previous_kernel();
   __shared__ double sums[32];
   double sum = 0.0;
 #pragma unroll 4
@@ -873,6 +909,8 @@ loss_weights_kernel(const float* upstream, int64_t upstream_stride, int per_row,
                     const int32_t* count, const int32_t* __restrict__ kept_index, float lift,
                     float* __restrict__ weight_of, float* gradient_scale, const void* targets,
                     int targets_64, int64_t ignored, int64_t N, unsigned short* dhidden, int D) {
+  start_next_kernel();
+  wait_for_previous_kernel();
   const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
     if (dhidden == nullptr) return;

@@ -186,8 +186,8 @@ extern "C" int attnres_b200_norm_backward(
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   if (int st = dispatch_norm_type<kBackward>(p, type, vector, sms, cs)) return st;
   if (!want_params) return ATTNRES_B200_OK;
-  layer_norm_param_reduce_kernel<<<(2 * D + kNormReduceColumns - 1) / kNormReduceColumns,
-                                   kNormReduceColumns * kNormReduceGroups, 0, cs>>>(
-      partials, grid, D, dweight, dbias, param_type);
-  return launched();
+  return launch_behind(layer_norm_param_reduce_kernel,
+                       (2 * D + kNormReduceColumns - 1) / kNormReduceColumns,
+                       kNormReduceColumns * kNormReduceGroups, 0, true, cs, (const float*)partials,
+                       grid, D, dweight, dbias, param_type);
 }

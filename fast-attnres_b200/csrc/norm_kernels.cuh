@@ -302,6 +302,7 @@ layer_norm_fwd_kernel(const NormParams p) {
 template <typename T, bool VECTOR, int E, int WARPS>
 __global__ void __launch_bounds__(kNormThreads, norm_grad_ctas(E))
 layer_norm_grad_kernel(const NormParams p) {
+  start_next_kernel();  // the reduction of the partial sums waits for the end
   using Shape = NormShape<T, VECTOR, E, WARPS>;
   using Ring = NormRing<Shape, 2>;
   constexpr int TG = Shape::kThreads, GROUPS = kNormThreads / TG;
@@ -432,6 +433,7 @@ __global__ void __launch_bounds__(kNormReduceColumns * kNormReduceGroups)
 layer_norm_param_reduce_kernel(const float* __restrict__ partials, int rows, int D, void* dweight,
                                void* dbias, int param_type) {
   __shared__ double sums[kNormReduceGroups][kNormReduceColumns + 1];
+  wait_for_previous_kernel();
   const int col = threadIdx.x % kNormReduceColumns, grp = threadIdx.x / kNormReduceColumns;
   const int c = blockIdx.x * kNormReduceColumns + col;
   double s[4] = {0.0, 0.0, 0.0, 0.0};

@@ -196,8 +196,27 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 };
 
+// Whether a call has to leave a node behind.  Without one it goes straight to the device's (or the
+// tracer's) kernel.
+bool differentiated(std::initializer_list<const Tensor*> inputs) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : inputs)
+    if (t != nullptr && t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+const Tensor* given(const optional<Tensor>& t) { return t.has_value() ? &*t : nullptr; }
+
+Tensor layer_norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias,
+                  double eps);
+
 Tensor layer_norm_autograd(const Tensor& x, const optional<Tensor>& weight,
                            const optional<Tensor>& bias, double eps) {
+  if (!differentiated({&x, given(weight), given(bias)})) {
+    static auto op = operation<decltype(layer_norm)>("attnres_b200::layer_norm");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(x, weight, bias, eps);
+  }
   return LayerNorm::apply(x, weight, bias, eps);
 }
 
@@ -307,8 +326,16 @@ struct Embed : torch::autograd::Function<Embed> {
   }
 };
 
+Tensor embed(const Tensor& tokens, const Tensor& table, const optional<Tensor>& positions,
+             double scale, int64_t padding, ScalarType type);
+
 Tensor embed_autograd(const Tensor& tokens, const Tensor& table, const optional<Tensor>& positions,
                       double scale, int64_t padding, ScalarType type) {
+  if (!differentiated({&table, given(positions)})) {
+    static auto op = operation<decltype(embed)>("attnres_b200::embed");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(tokens, table, positions, scale, padding, type);
+  }
   return Embed::apply(tokens, table, positions, scale, padding, type);
 }
 
@@ -498,8 +525,16 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
   }
 };
 
+Tensor loss(const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignored,
+            int64_t reduction, double scale);
+
 Tensor loss_autograd(const Tensor& hidden, const Tensor& weight, const Tensor& targets,
                      int64_t ignored, int64_t reduction, double scale) {
+  if (!differentiated({&hidden, &weight})) {
+    static auto op = operation<decltype(loss)>("attnres_b200::linear_cross_entropy");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(hidden, weight, targets, ignored, reduction, scale);
+  }
   return LinearCrossEntropy::apply(hidden, weight, targets, ignored, reduction, scale);
 }
 

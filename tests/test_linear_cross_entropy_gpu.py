@@ -124,10 +124,14 @@ def test_linear_cross_entropy_matches_the_definition(rows, vocabulary, width, dt
 
 @pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("rows,vocabulary,width", [
-    (2500, 6001, 136),      # pairs of CTAs for the logits, single ones for the gradients
-    (3001, 20003, 264),     # pairs for both
+    (2500, 6001, 136),
+    (5200, 6001, 136),      # pairs of CTAs for the logits, single ones for the gradients
+    (3001, 20003, 264),
+    (5500, 35003, 264),     # pairs for both
     (200, 30000, 40),       # dH in slices of the vocabulary
-    (2900, 20003, 517)])    # pairs, element-wise rows
+    (200, 30000, 1100),     # logits in two segments of the features
+    (2900, 20003, 517),
+    (5500, 20003, 1029)])   # pairs, element-wise rows, segments
 def test_linear_cross_entropy_every_kind_of_product(rows, vocabulary, width, dtype):
     hidden, weight, targets = _case(rows, vocabulary, width, dtype, ignored=0.1, seed=14)
     first = _check(hidden, weight, targets)
