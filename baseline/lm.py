@@ -16,6 +16,11 @@ reference's "sliced" variant) and goes through an injected ``operator(values, qu
 this library, the reference's Triton package and the oracle all drive the same network.
 Parameter names follow the reference model so state dicts are interchangeable.
 
+The three operators at the ends of the network can be injected as well (``ends``, an ``Ends``): the
+embedding that makes the first source, the LayerNorm of sublayers whose norm does not ride on a
+read, and the head with its loss, which then never forms the logits of a whole batch
+(``library_ends()`` gives this library's).
+
 This file is benchmark and test scaffolding (used by bench.py's model workloads,
 baseline/train_step_ab.py and tests/test_lm_schedule.py), not part of the operator package.
 """
@@ -137,14 +142,33 @@ class _Layer(nn.Module):
         return self.mlp_from_normed(self.norm_mlp(x))
 
 
+@dataclass(frozen=True)
+class Ends:
+    """``embed(tokens, table, positions, *, dtype)``, ``layer_norm(x, weight, bias, eps)`` and
+    ``loss(hidden, head_weight, targets)`` (the mean over the targets)."""
+    embed: object
+    layer_norm: object
+    loss: object
+
+
+def library_ends() -> Ends:
+    from attnres.embedding import embed
+    from attnres.loss import linear_cross_entropy
+    from attnres.norm import layer_norm
+    return Ends(embed, layer_norm, linear_cross_entropy)
+
+
 class CausalLM(nn.Module):
     """``operator(values, query)`` is any implementation of the read; ``normed_operator``,
     when given, is ``(values, query, weight, bias, norm_eps) -> LayerNorm(read)`` and replaces
-    the read + LayerNorm pair in front of every sublayer (the fused epilogue)."""
+    the read + LayerNorm pair in front of every sublayer (the fused epilogue).  ``ends``, when
+    given, holds the operators that replace embedding, LayerNorm and head with loss; the model is
+    then also called as ``model(tokens, targets)`` and returns the mean loss."""
 
-    def __init__(self, config: LMConfig, operator, normed_operator=None):
+    def __init__(self, config: LMConfig, operator, normed_operator=None, ends: Ends | None = None):
         super().__init__()
         self.config, self.operator, self.normed_operator = config, operator, normed_operator
+        self.ends = ends
         self.token_embedding = nn.Embedding(config.vocab, config.width)
         self.position_embedding = nn.Parameter(torch.empty(config.sequence, config.width))
         self.layers = nn.ModuleList(_Layer(config) for _ in range(config.layers))
@@ -162,11 +186,26 @@ class CausalLM(nn.Module):
         """The first source, in the working dtype of the residual stream: the autocast dtype
         when autocast is on, else the parameters' (benchmarks/model.py:239-245 of the reference).
         Reads always see BF16 and return the working dtype."""
+        if self.ends is not None:
+            return self.ends.embed(tokens, self.token_embedding.weight,
+                                   self.position_embedding[: tokens.shape[-1]],
+                                   dtype=self._working_dtype())
         embedded = self.token_embedding(tokens) + self.position_embedding[: tokens.shape[-1]]
         device_type = embedded.device.type
         if torch.is_autocast_enabled(device_type):
             embedded = embedded.to(torch.get_autocast_dtype(device_type))
         return embedded
+
+    def _working_dtype(self):
+        weight = self.token_embedding.weight
+        if torch.is_autocast_enabled(weight.device.type):
+            return torch.get_autocast_dtype(weight.device.type)
+        return weight.dtype
+
+    def _norm(self, norm, x):
+        if self.ends is None:
+            return norm(x)
+        return self.ends.layer_norm(x, norm.weight, norm.bias, norm.eps)
 
     def _values(self, sources):
         sources = tuple(s.to(torch.bfloat16) for s in sources)
@@ -182,21 +221,26 @@ class CausalLM(nn.Module):
         norm = layer.norm_attention if event % 2 == 0 else layer.norm_mlp
         body = layer.attention_from_normed if event % 2 == 0 else layer.mlp_from_normed
         if event == 0:
-            return body(norm(sources[0]))
+            return body(self._norm(norm, sources[0]))
         if self.normed_operator is not None:
             normed = self.normed_operator(self._values(sources),
                                           self.queries[event - 1].to(torch.bfloat16),
                                           norm.weight, norm.bias, norm.eps)
             return body(normed.to(norm.weight.dtype)
                         if not torch.is_autocast_enabled(normed.device.type) else normed)
-        return body(norm(self.read(sources, event - 1)))
+        return body(self._norm(norm, self.read(sources, event - 1)))
 
-    def forward(self, tokens):
+    def forward(self, tokens, targets=None):
+        """Logits; with ``targets`` (and ``ends``) the mean loss."""
         config = self.config
         schedule = SourceSchedule(self.embed(tokens), config.events, config.block_count)
         for event in range(config.events):
             schedule.emit(self.sublayer(event, schedule.sources()))
-        return self.lm_head(self.read(schedule.sources(), config.events - 1))
+        last = self.read(schedule.sources(), config.events - 1)
+        if targets is None:
+            return self.lm_head(last)
+        last = last.to(self._working_dtype())
+        return self.ends.loss(last, self.lm_head.weight.to(last.dtype), targets)
 
 
 def make_optimizer(model, *, capturable: bool, lr: float = 3e-4):
@@ -205,10 +249,12 @@ def make_optimizer(model, *, capturable: bool, lr: float = 3e-4):
                              fused=True, capturable=capturable)
 
 
-def training_step(model, optimizer, tokens, targets, *, accumulation: int = 1, sync_context=None):
+def training_step(model, optimizer, tokens, targets, *, accumulation: int = 1, sync_context=None,
+                  loss_in_model: bool = False):
     """zero_grad, BF16-autocast forward, cross entropy, backward over `accumulation`
     microbatches, optimiser step (benchmarks/training_graph.py:24-58 of the reference).
-    ``sync_context(last)`` may return a context manager per microbatch (DDP's ``no_sync``)."""
+    ``sync_context(last)`` may return a context manager per microbatch (DDP's ``no_sync``);
+    ``loss_in_model``: the model was given ``ends`` and forms the loss itself."""
     import contextlib
     optimizer.zero_grad(set_to_none=False)
     loss = None
@@ -218,9 +264,12 @@ def training_step(model, optimizer, tokens, targets, *, accumulation: int = 1, s
                    else contextlib.nullcontext())
         with context:
             with torch.autocast("cuda" if tokens.is_cuda else "cpu", dtype=torch.bfloat16):
-                logits = model(micro_tokens)
-                loss = F.cross_entropy(logits.reshape(-1, logits.shape[-1]),
-                                       micro_targets.reshape(-1))
+                if loss_in_model:
+                    loss = model(micro_tokens, micro_targets)
+                else:
+                    logits = model(micro_tokens)
+                    loss = F.cross_entropy(logits.reshape(-1, logits.shape[-1]),
+                                           micro_targets.reshape(-1))
             (loss / accumulation).backward()
     optimizer.step()
     return loss.detach()

@@ -24,6 +24,8 @@ Arms (every arm is its own process, because both packages are called ``attnres``
 * ``ours-packed``    this library, ``torch.stack`` then the packed operator;
 * ``ours-fused``     this library, list layout, the LayerNorm in front of every sublayer
                      computed in the read's epilogue (``attnres.fused.attnres_layer_norm``);
+* ``ours-ends``      this library, list layout, and its embedding, LayerNorm and head with loss at
+                     the ends of the network (``baseline/lm.py::library_ends``);
 * ``ours-accumulate`` this library, list layout, staged backward: every read takes detached
                      sources and its backward kernel adds the value gradients into one running
                      buffer per sublayer output (``attnres.accumulate.attnres_accumulate``);
@@ -45,11 +47,13 @@ import time
 from pathlib import Path
 
 ROOT = Path(__file__).resolve().parents[1]
-ARMS = ("triton-list", "triton-packed", "ours-list", "ours-packed", "ours-fused", "ours-accumulate")
+ARMS = ("triton-list", "triton-packed", "ours-list", "ours-packed", "ours-fused", "ours-ends",
+        "ours-accumulate")
 # `--arm all` without `--arms` runs these; `ours-fused` is selectable by name (its set-up under
 # torch.compile has taken minutes in this harness for a reason not found, while a stand-alone
 # compile of the same model takes seconds).
-DEFAULT_ARMS = ("triton-list", "triton-packed", "ours-list", "ours-packed", "ours-accumulate")
+DEFAULT_ARMS = ("triton-list", "triton-packed", "ours-list", "ours-packed", "ours-ends",
+                "ours-accumulate")
 
 
 def staged_step_factory(torch, model, lm, accumulate, buffers, optimizer, tokens, targets,
@@ -118,7 +122,8 @@ def run_arm(arm: str, steps: int, layers: int, batch: int, sequence: int, compil
         from attnres.fused import attnres_layer_norm
         normed = attnres_layer_norm
     with torch.device(device):
-        model = lm.CausalLM(config, package.attnres, normed_operator=normed)
+        model = lm.CausalLM(config, package.attnres, normed_operator=normed,
+                            ends=lm.library_ends() if layout == "ends" else None)
     optimizer = lm.make_optimizer(model, capturable=True)
     tokens = torch.randint(config.vocab, (batch, sequence), device=device)
     targets = torch.randint(config.vocab, (batch, sequence), device=device)
@@ -132,7 +137,8 @@ def run_arm(arm: str, steps: int, layers: int, batch: int, sequence: int, compil
         runner = torch.compile(model, fullgraph=True, dynamic=False) if compiled else model
 
         def step():
-            return lm.training_step(runner, optimizer, tokens, targets)
+            return lm.training_step(runner, optimizer, tokens, targets,
+                                    loss_in_model=layout == "ends")
 
     captured = lm.CapturedStep(step, model, optimizer, warmup=3)
     ready = time.perf_counter()

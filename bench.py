@@ -774,7 +774,7 @@ def run_model_workload(args, rank: int, world: int, local_rank: int) -> None:
     config = lm.LMConfig(**spec)
     torch.manual_seed(SEED)            # the same initial weights on every rank
     with torch.device(device):
-        model = lm.CausalLM(config, attnres)
+        model = lm.CausalLM(config, attnres, ends=lm.library_ends() if args.ends else None)
     if parameters == "bf16":
         model = model.to(torch.bfloat16)
     wrapped = model
@@ -809,7 +809,7 @@ def run_model_workload(args, rank: int, world: int, local_rank: int) -> None:
         loss = None
         for _ in range(steps):
             loss = lm.training_step(runner, optimizer, tokens, targets, accumulation=accumulation,
-                                    sync_context=context)
+                                    sync_context=context, loss_in_model=args.ends)
         stop.record()
         if distributed:
             dist.barrier()
@@ -852,7 +852,7 @@ def run_model_workload(args, rank: int, world: int, local_rank: int) -> None:
                    "global_batch_sequences": batch_per_gpu * accumulation * world,
                    "parameters": parameters, "parameter_count": parameters_count,
                    "optimizer": f"AdamW fused lr {learning_rate:g} betas 0.9/0.95 wd 0.1",
-                   "compiled": bool(args.compile),
+                   "compiled": bool(args.compile), "library_ends": bool(args.ends),
                    "parallelism": f"data parallel x{world} (DistributedDataParallel, NCCL, "
                                   "256 MB buckets overlapping the backward)",
                    "reads_per_microbatch": len(counts), "sources_per_read": sorted(set(counts)),
@@ -1046,6 +1046,9 @@ def main() -> None:
                              "global batch of 32 sequences")
     parser.add_argument("--compile", action="store_true",
                         help="model workloads: run the model under torch.compile")
+    parser.add_argument("--ends", action="store_true",
+                        help="model workloads: this library's embedding, LayerNorm and head with "
+                             "loss instead of the framework's")
     parser.add_argument("--cell", default=None, help="S,D[,R]: time one shape instead of the sweep")
     parser.add_argument("--rows", type=int, default=ROWS, help="rows of the --cell run")
     parser.add_argument("--generic", action="store_true", help="--cell: force the generic kernels")

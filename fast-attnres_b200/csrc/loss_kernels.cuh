@@ -77,7 +77,8 @@ constexpr int kGatherThreads = 1024;
 
 template <bool VECTOR>
 __global__ void __launch_bounds__(kGatherThreads) loss_gather_kernel(const GatherParams p) {
-  start_next_kernel();
+  // With more than a CTA to an SM the waiting kernel would take room that the gathering needs.
+  if (gridDim.x <= 148) start_next_kernel();
   wait_for_previous_kernel();
   __shared__ int warp_counts[kGatherThreads / 32];
   __shared__ int places[kGatherThreads];
@@ -819,13 +820,16 @@ loss_join_kernel(const float2* __restrict__ partials, int pairs, const int32_t* 
   }
 }
 
-// The same, and the row's codes become P = p - [v = target] in place.
+// The same, and the row's codes become P = p - [v = target] in place.  Memory bounds it: 4 bytes a
+// logit, 4.7 TB/s at 16 384 x 32 000 (445 us; taking the rows last first, for what L2 still holds
+// of them, was slower).
 __global__ void __launch_bounds__(kJoinThreads)
 loss_probs_kernel(const float2* __restrict__ partials, int pairs, const int32_t* count, int first_row,
                   int row_limit, const float* __restrict__ target_logit,
                   const int32_t* __restrict__ kept_target, const int32_t* __restrict__ kept_index,
                   float* __restrict__ losses, unsigned short* codes, int64_t stride, int V) {
-  start_next_kernel();
+  // (The products' CTAs would take the L1 cache for their shared memory while they wait: they start
+  // when this kernel's CTAs are done.)
   wait_for_previous_kernel();
   const int tid = threadIdx.x, rows = min(max(*count - first_row, 0), row_limit);
   for (int row = blockIdx.x; row < rows; row += gridDim.x) {
