@@ -1,6 +1,5 @@
 // C ABI of the vocabulary loss (declared in include/attnres_b200.h).
 #include <cmath>
-#include <mutex>
 
 #include "loss_kernels.cuh"
 
@@ -27,10 +26,10 @@ namespace {
 
 constexpr int64_t kMaxLossRows = 1 << 30;
 constexpr int32_t kMaxLossVocabulary = 1 << 25;
-// Rows whose (max, sum) pairs are held at a time (65 536 x 250 pairs at 32 000 ids: 131 MB).
-constexpr int64_t kStatsRows = 65536;
-// Bytes of P held at a time.  More pieces mean more FP32 parts of a gradient to add; 16 384 rows of
-// 32 000 ids are one piece.
+// Bytes of (max, sum) pairs held at a time (65 536 rows of 32 000 ids take 131 MB).
+constexpr int64_t kPairBytes = 256ll << 20;
+// Bytes of P held at a time.  With more than one piece a gradient is added up in FP32 in memory;
+// 16 384 rows of 32 000 ids are one piece.
 constexpr int64_t kPieceBytes = 1024ll << 20;
 constexpr int64_t kPieceMinimum = 4096;
 
@@ -39,19 +38,19 @@ typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, v
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+EncodeTiled find_encode_tiled() {
+  void* found = nullptr;
+  cudaDriverEntryPointQueryResult result;
+  if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &found, 12000, cudaEnableDefault,
+                                       &result) == cudaSuccess &&
+      result == cudaDriverEntryPointSuccess)
+    return reinterpret_cast<EncodeTiled>(found);
+  cudaGetLastError();
+  return nullptr;
+}
+
 EncodeTiled encode_tiled() {
-  static std::once_flag once;
-  static EncodeTiled function = nullptr;
-  std::call_once(once, [] {
-    void* found = nullptr;
-    cudaDriverEntryPointQueryResult result;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &found, 12000, cudaEnableDefault,
-                                         &result) == cudaSuccess &&
-        result == cudaDriverEntryPointSuccess)
-      function = reinterpret_cast<EncodeTiled>(found);
-    else
-      cudaGetLastError();
-  });
+  static const EncodeTiled function = find_encode_tiled();
   return function;
 }
 
@@ -109,8 +108,10 @@ bool use_pairs(int64_t tiles_of_pairs) { return tiles_of_pairs >= 296; }
 LossPlan plan_loss(int64_t N, int32_t V, int32_t D) {
   LossPlan plan;
   plan.padded_weight = align256((int64_t)V * padded_width(D) * 2);
-  plan.stats_rows = N < kStatsRows ? N : kStatsRows;
   const int64_t tiles_n = (V + kTileN - 1) / kTileN;
+  plan.stats_rows = kPairBytes / (2 * tiles_n * (int64_t)sizeof(float2)) / 256 * 256;
+  if (plan.stats_rows < 256) plan.stats_rows = 256;
+  if (plan.stats_rows > N) plan.stats_rows = N;
   plan.partials = align256(plan.stats_rows * 2 * tiles_n * (int64_t)sizeof(float2));
   int64_t most = kPieceBytes / (2 * N) / kTileN * kTileN;
   if (most < kPieceMinimum) most = kPieceMinimum;
@@ -125,8 +126,9 @@ LossPlan plan_loss(int64_t N, int32_t V, int32_t D) {
   plan.slices = 148 / tiles;
   if (plan.slices > steps / 16) plan.slices = steps / 16;
   if (plan.slices < 1) plan.slices = 1;
-  const int64_t all = plan.slices * plan.pieces;
-  plan.slices_out = all > 1 ? align256(all * N * D * (int64_t)sizeof(float)) : 0;
+  plan.slices_out = plan.slices * plan.pieces > 1
+                        ? align256(plan.slices * N * D * (int64_t)sizeof(float))
+                        : 0;
   plan.weights = align256((N + 1) * (int64_t)sizeof(float));
   return plan;
 }
@@ -134,13 +136,13 @@ LossPlan plan_loss(int64_t N, int32_t V, int32_t D) {
 // The forward that forms the gradients as well works on pieces of the rows.
 struct GradientPlan {
   int64_t piece, pieces;  // rows
-  int64_t partials, codes, weight_parts;
+  int64_t partials, codes, weight_out;
 };
 
 GradientPlan plan_gradients(int64_t N, int32_t V, int32_t D) {
   GradientPlan plan;
   int64_t most = kPieceBytes / (2 * (int64_t)padded_width(V)) / 256 * 256;
-  if (most < 1024) most = 1024;
+  if (most < 256) most = 256;
   plan.pieces = (N + most - 1) / most;
   plan.piece = ((N + plan.pieces - 1) / plan.pieces + 255) / 256 * 256;
   if (plan.piece > N) plan.piece = N;
@@ -148,8 +150,7 @@ GradientPlan plan_gradients(int64_t N, int32_t V, int32_t D) {
   const int64_t tiles_n = (V + kTileN - 1) / kTileN;
   plan.partials = align256(plan.piece * 2 * tiles_n * (int64_t)sizeof(float2));
   plan.codes = align256(plan.piece * (int64_t)padded_width(V) * 2);
-  plan.weight_parts =
-      plan.pieces > 1 ? align256(plan.pieces * V * (int64_t)D * (int64_t)sizeof(float)) : 0;
+  plan.weight_out = plan.pieces > 1 ? align256((int64_t)V * D * (int64_t)sizeof(float)) : 0;
   return plan;
 }
 
@@ -222,7 +223,7 @@ extern "C" int64_t attnres_b200_loss_workspace_bytes(int64_t N, int32_t V, int32
   if (pass == ATTNRES_B200_LOSS_FORWARD_GRADIENTS) {
     const GradientPlan gradients = plan_gradients(N, V, D);
     return plan.padded_weight + gradients.partials + logits + 256 + gradients.codes +
-           gradients.weight_parts;
+           gradients.weight_out;
   }
   if (pass != ATTNRES_B200_LOSS_BACKWARD) return -ATTNRES_B200_ERR_BAD_FLAGS;
   return plan.padded_weight + plan.probs + plan.slices_out + plan.weights;
@@ -265,7 +266,7 @@ extern "C" int attnres_b200_loss_forward(
   rest += align256(N * (int64_t)sizeof(float));
   float* gradient_scale = reinterpret_cast<float*>(rest);  // from here on with gradients only
   unsigned short* codes = reinterpret_cast<unsigned short*>(rest + 256);
-  float* weight_parts = reinterpret_cast<float*>(rest + 256 + pieces.codes);
+  float* weight_out = reinterpret_cast<float*>(rest + 256 + pieces.codes);
 
   GatherParams g{};
   g.hidden = hidden;
@@ -336,7 +337,8 @@ extern "C" int attnres_b200_loss_forward(
                                  p.row_limit, target_logit, kept_target, kept_index, losses, codes,
                                  stride, V))
         return st;
-      p.weight_out = dweight != nullptr && pieces.pieces > 1 ? weight_parts + piece * V * D : nullptr;
+      p.weight_out = dweight != nullptr && pieces.pieces > 1 ? weight_out : nullptr;
+      p.add = piece > 0;
       const auto both = [&](bool pair) {
         return (dhidden ? tiles_of(p.row_limit, D, pair) : 0) + (dweight ? tiles_of(V, D, pair) : 0);
       };
@@ -344,7 +346,7 @@ extern "C" int attnres_b200_loss_forward(
     }
     if (p.weight_out != nullptr) {
       if (int st = launch_behind(loss_slices_kernel<__nv_bfloat16>, 8 * sms, 256, 0, true, cs,
-                                 weight_parts, (int)pieces.pieces, nullptr, nullptr, gradient_scale,
+                                 weight_out, 1, nullptr, nullptr, gradient_scale,
                                  scale, (int64_t)V, D, static_cast<__nv_bfloat16*>(dweight),
                                  p.vector_dweight))
         return st;
@@ -442,16 +444,16 @@ extern "C" int attnres_b200_loss_backward(
              (dweight ? tiles_of(p.vn, D, pair) : 0);
     };
     if (int st = launch_product_type<kGradients>(type, use, p, gradients, sms, cs)) return st;
-    p.first_slice += p.slices;
+    p.add = 1;
   }
   if (dhidden == nullptr || p.slices_out == nullptr) return ATTNRES_B200_OK;
   const int64_t ctas = (N + 7) / 8;
   const unsigned grid = (unsigned)(ctas < 8 * sms ? ctas : 8 * sms);
   if (type == ATTNRES_B200_BF16)
     return launch_behind(loss_slices_kernel<__nv_bfloat16>, grid, 256, 0, true, cs, slices_out,
-                         p.first_slice, count, kept_index, gradient_scale, scale, N, D,
+                         p.slices, count, kept_index, gradient_scale, scale, N, D,
                          static_cast<__nv_bfloat16*>(dhidden), p.vector_dhidden);
-  return launch_behind(loss_slices_kernel<__half>, grid, 256, 0, true, cs, slices_out, p.first_slice,
+  return launch_behind(loss_slices_kernel<__half>, grid, 256, 0, true, cs, slices_out, p.slices,
                        count, kept_index, gradient_scale, scale, N, D, static_cast<__half*>(dhidden),
                        p.vector_dhidden);
 }

@@ -201,10 +201,10 @@ struct ProductParams {
   const float* gradient_scale;  // kGradients
   void* dhidden;           // kGradients: [N, D] or NULL
   void* dweight;           // kGradients: [V, D] or NULL
-  float* slices_out;       // dH in several slices of the vocabulary: FP32 [slices][N, D]
-  int32_t first_slice;     // of this piece
-  int32_t slices;          // that this piece is cut into
-  float* weight_out;       // dW from several pieces of the rows: FP32 [V, D] of this piece
+  float* slices_out;       // dH in several slices of the vocabulary: FP32 [slices][N, D], or NULL
+  int32_t slices;          // that a piece's sum for dH is cut into
+  float* weight_out;       // dW from several pieces of the rows: FP32 [V, D], or NULL
+  int32_t add;             // not the first piece: slices_out and weight_out are added to
   int32_t vector_dhidden, vector_dweight;  // their rows allow 16-byte stores
 };
 
@@ -247,10 +247,10 @@ __device__ __forceinline__ uint32_t block_slot(uint32_t staging, int row, int ch
 
 // Writes the block out row by row, so that a store covers whole lines: `mine` is the element offset
 // in `out` of this lane's row, or negative when that row has no place; `columns` (of 128 bytes'
-// worth) are valid.
+// worth) are valid.  `add` (FP32 only) adds to what is there.
 template <typename T>
 __device__ __forceinline__ void write_block(uint32_t staging, T* out, int64_t mine, int columns,
-                                            bool vector, int lane) {
+                                            bool vector, int lane, bool add = false) {
   constexpr int per_chunk = 16 / (int)sizeof(T), width = 8 * per_chunk;
   __syncwarp();
   if (vector) {
@@ -258,9 +258,18 @@ __device__ __forceinline__ void write_block(uint32_t staging, T* out, int64_t mi
     for (int i = 0; i < 8; ++i) {
       const int row = i * 4 + (lane >> 3), chunk = lane & 7;
       const int64_t offset = __shfl_sync(0xffffffffu, mine, row);
-      if (offset >= 0 && chunk * per_chunk < columns)
-        *reinterpret_cast<uint4*>(out + offset + chunk * per_chunk) =
-            load_shared16(block_slot(staging, row, chunk));
+      if (offset >= 0 && chunk * per_chunk < columns) {
+        uint4* place = reinterpret_cast<uint4*>(out + offset + chunk * per_chunk);
+        uint4 v = load_shared16(block_slot(staging, row, chunk));
+        if (sizeof(T) == 4 && add) {
+          const uint4 there = *place;
+          v.x = __float_as_uint(__uint_as_float(there.x) + __uint_as_float(v.x));
+          v.y = __float_as_uint(__uint_as_float(there.y) + __uint_as_float(v.y));
+          v.z = __float_as_uint(__uint_as_float(there.z) + __uint_as_float(v.z));
+          v.w = __float_as_uint(__uint_as_float(there.w) + __uint_as_float(v.w));
+        }
+        *place = v;
+      }
     }
   } else {
     for (int row = 0; row < 32; ++row) {
@@ -275,6 +284,7 @@ __device__ __forceinline__ void write_block(uint32_t staging, T* out, int64_t mi
           if constexpr (sizeof(T) == 4) {
             float v;
             asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(slot) : "memory");
+            if (add) v = (float)out[offset + column] + v;
             out[offset + column] = v;
           } else {
             unsigned short v;
@@ -641,12 +651,12 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
                 make_float2(top, sums[0] + sums[1]);
         }
       } else if ((t.weight ? p.weight_out : p.slices_out) != nullptr) {
-        // A part of the sum: FP32, added to the others by loss_slices_kernel.
+        // A part of the sum, in FP32: loss_slices_kernel adds the slices and rounds.
         int64_t place = -1;
         if (t.weight) {
           if (row < p.vn) place = (int64_t)(p.v0 + row) * p.D + column;
         } else if (row < kept) {
-          place = ((int64_t)(p.first_slice + t.slice) * p.N + row) * p.D + column;
+          place = ((int64_t)t.slice * p.N + row) * p.D + column;
         }
         float* parts = t.weight ? p.weight_out : p.slices_out;
 #pragma unroll 1
@@ -661,7 +671,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
             else
               store_shared16(block_slot(staging, lane, q), 0u, 0u, 0u, 0u);
           }
-          write_block<float>(staging, parts + c, place, columns - c, p.D % 4 == 0, lane);
+          write_block<float>(staging, parts + c, place, columns - c, p.D % 4 == 0, lane, p.add);
         }
       } else {
         int64_t place = -1;

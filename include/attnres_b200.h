@@ -393,7 +393,7 @@ int attnres_b200_embedding_backward(
  *                    one of the three below
  *
  * No pass holds more of [N,V] than one piece, 16 bits an element: 1 GiB, or 4096 ids (backward) or
- * 1024 rows (forward with gradients) where that is more.  Results are the same bits every time.
+ * 256 rows (forward with gradients) where that is more.  Results are the same bits every time.
  */
 #define ATTNRES_B200_LOSS_NONE 0
 #define ATTNRES_B200_LOSS_SUM 1

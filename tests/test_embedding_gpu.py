@@ -272,3 +272,25 @@ def test_embed_writes_only_its_outputs():
         for whole in (out_all, dt_all, dp_all, ws_all):
             assert bool((whole[:pad] == -7).all()) and bool((whole[-pad:] == -7).all())
         assert torch.equal(out.view(n, width), table[tokens])
+
+
+def test_embed_on_two_streams_in_inference_mode_and_twice():
+    """Two gradients at once, each with its own workspace; and no second derivative."""
+    from attnres.embedding import embed
+    tables = [_table(3000, 264, FP32, seed).requires_grad_() for seed in (1, 2)]
+    tokens = [_ids((4, 700), 3000, seed) for seed in (3, 4)]
+    upstream = torch.randn(4, 700, 264, device="cuda")
+    want = [torch.autograd.grad(embed(t, w), w, upstream)[0] for t, w in zip(tokens, tables)]
+    with torch.inference_mode():
+        assert torch.equal(embed(tokens[0], tables[0]), tables[0][tokens[0]])
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(torch.autograd.grad(embed(tokens[i], tables[i]), tables[i], upstream)[0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+    grad, = torch.autograd.grad(embed(tokens[0], tables[0]).sum(), tables[0], create_graph=True)
+    with pytest.raises(RuntimeError):
+        grad.sum().backward()

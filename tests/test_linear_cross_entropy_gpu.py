@@ -302,9 +302,12 @@ def test_linear_cross_entropy_strange_upstream_weights_stay_with_their_rows():
 
 @pytest.mark.parametrize("rows,vocabulary,width,ignored", [
     (40000, 8200, 64, 0.0),
-    (66000, 4999, 40, 0.2),      # two blocks of rows
-    (70000, 8300, 40, 0.2),      # and two pieces of the vocabulary, the last of them short
+    (66000, 4999, 40, 0.2),
+    (9000, 140000, 24, 0.2),     # logits in blocks of rows, three pieces of the vocabulary
+    (70000, 8300, 40, 0.2),      # two pieces of the vocabulary, the last of them short
+    (70000, 8300, 39, 0.0),
     (66500, 8300, 512, 0.1),     # gradients in the forward, two pieces of the rows
+    (66500, 8301, 515, 0.0),
 ])
 def test_linear_cross_entropy_in_pieces(rows, vocabulary, width, ignored):
     hidden, weight, targets = _case(rows, vocabulary, width, BF16, ignored=ignored, seed=7)
@@ -470,6 +473,30 @@ def test_linear_cross_entropy_writes_only_its_outputs():
         torch.cuda.synchronize()
         for name, whole in buffers.items():
             assert bool((whole[:pad] == -7).all()) and bool((whole[-pad:] == -7).all()), name
+
+
+@pytest.mark.parametrize("width", [72, 520])
+def test_linear_cross_entropy_on_two_streams_in_inference_mode_and_twice(width):
+    """Two calls at once, each with its own workspace; and no second derivative."""
+    from attnres.loss import linear_cross_entropy
+    cases = [_case(700, 3000, width, BF16, ignored=0.2, seed=seed) for seed in (20, 21)]
+    leaves = [[h.requires_grad_(), w.requires_grad_()] for h, w, _ in cases]
+    call = lambda i: torch.autograd.grad(linear_cross_entropy(*leaves[i], cases[i][2]), leaves[i])  # noqa: E731
+    want = [call(i) for i in range(2)]
+    loss = linear_cross_entropy(*leaves[0], cases[0][2])
+    with torch.inference_mode():
+        assert torch.equal(linear_cross_entropy(*leaves[0], cases[0][2]), loss)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i in range(2) for g in got[i] for a, b in zip(g, want[i]))
+    grads = torch.autograd.grad(loss, leaves[0], create_graph=True)
+    with pytest.raises(RuntimeError):
+        grads[0].float().sum().backward()
 
 
 def test_no_product_gave_up_waiting():

@@ -111,6 +111,22 @@ def test_layer_norm_more_rows_than_one_pass_of_the_grid(rows, width, dtype):
     assert all(torch.equal(first[k], second[k]) for k in first), "not the same bits twice"
 
 
+def test_layer_norm_of_one_row_without_a_batch_axis_in_inference_mode_and_on_another_stream():
+    from attnres.norm import layer_norm
+    x, w, b, g = _case(1, 777, BF16, 16)
+    _check(x[0], w, b, g[0])
+    want = layer_norm(x, w, b).detach()
+    with torch.inference_mode():
+        assert torch.equal(layer_norm(x, w, b), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        results = [layer_norm(x, w, b).detach() for _ in range(20)]
+    mine = [layer_norm(x, w, b).detach() for _ in range(20)]   # at the same time, on this one
+    torch.cuda.synchronize()
+    assert all(torch.equal(r, want) for r in results + mine)
+
+
 @pytest.mark.parametrize("layout", ["padded", "odd offset", "transposed", "every other", "expanded",
                                     "three axes", "swapped axes"])
 def test_layer_norm_layouts(layout):
