@@ -222,7 +222,7 @@ extern "C" int64_t attnres_b200_loss_workspace_bytes(int64_t N, int32_t V, int32
   if (pass == ATTNRES_B200_LOSS_FORWARD) return plan.padded_weight + plan.partials + logits;
   if (pass == ATTNRES_B200_LOSS_FORWARD_GRADIENTS) {
     const GradientPlan gradients = plan_gradients(N, V, D);
-    return plan.padded_weight + gradients.partials + logits + 256 + gradients.codes +
+    return plan.padded_weight + gradients.partials + 2 * logits + 256 + gradients.codes +
            gradients.weight_out;
   }
   if (pass != ATTNRES_B200_LOSS_BACKWARD) return -ATTNRES_B200_ERR_BAD_FLAGS;
@@ -265,8 +265,10 @@ extern "C" int attnres_b200_loss_forward(
   float* target_logit = reinterpret_cast<float*>(rest);
   rest += align256(N * (int64_t)sizeof(float));
   float* gradient_scale = reinterpret_cast<float*>(rest);  // from here on with gradients only
-  unsigned short* codes = reinterpret_cast<unsigned short*>(rest + 256);
-  float* weight_out = reinterpret_cast<float*>(rest + 256 + pieces.codes);
+  float* sums = gradient_scale + 64;
+  rest += 256 + align256(N * (int64_t)sizeof(float));
+  unsigned short* codes = reinterpret_cast<unsigned short*>(rest);
+  float* weight_out = reinterpret_cast<float*>(rest + pieces.codes);
 
   GatherParams g{};
   g.hidden = hidden;
@@ -332,10 +334,14 @@ extern "C" int attnres_b200_loss_forward(
       if (int st = make_map(&use[0], codes, type, p.row_limit, V, stride, 64)) return st;
       const auto logits = [&](bool pair) { return tiles_of(p.row_limit, V, pair); };
       if (int st = launch_product_type<kCodes>(type, form, p, logits, sms, cs)) return st;
-      if (int st = launch_behind(loss_probs_kernel, p.row_limit < 8 * sms ? p.row_limit : 8 * sms,
-                                 kJoinThreads, 0, true, cs, partials, pairs, count, p.first_row,
-                                 p.row_limit, target_logit, kept_target, kept_index, losses, codes,
-                                 stride, V))
+      if (int st = launch_behind(loss_join_kernel, (p.row_limit + 7) / 8, kJoinThreads, 0, true, cs,
+                                 partials, pairs, count, p.first_row, p.row_limit, target_logit,
+                                 kept_index, sums, losses))
+        return st;
+      const int64_t parts = (V + kProbsColumns - 1) / kProbsColumns;
+      if (int st = launch_behind(loss_probs_kernel, p.row_limit * parts, kProbsThreads, 0, true, cs,
+                                 partials, pairs, count, p.first_row, p.row_limit, target_logit,
+                                 kept_target, sums, codes, stride, V))
         return st;
       p.weight_out = dweight != nullptr && pieces.pieces > 1 ? weight_out : nullptr;
       p.add = piece > 0;
@@ -357,9 +363,9 @@ extern "C" int attnres_b200_loss_forward(
     p.row_limit = (int32_t)(N - row < plan.stats_rows ? N - row : plan.stats_rows);
     const auto tiles = [&](bool pair) { return tiles_of(p.row_limit, V, pair); };
     if (int st = launch_product_type<kStats>(type, maps, p, tiles, sms, cs)) return st;
-    if (int st = launch_behind(loss_join_kernel, p.row_limit < 8 * sms ? p.row_limit : 8 * sms,
-                               kJoinThreads, 0, true, cs, partials, pairs, count, p.first_row,
-                               p.row_limit, target_logit, kept_index, lse2, losses))
+    if (int st = launch_behind(loss_join_kernel, (p.row_limit + 7) / 8, kJoinThreads, 0, true, cs,
+                               partials, pairs, count, p.first_row, p.row_limit, target_logit,
+                               kept_index, lse2, losses))
       return st;
   }
   if (reduction == ATTNRES_B200_LOSS_NONE) return ATTNRES_B200_OK;

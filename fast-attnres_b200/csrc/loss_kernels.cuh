@@ -16,7 +16,7 @@
 //   kCodes      a piece of the rows: (max, sum) pairs as above, and z as 16-bit codes, the distance
 //               from the half tile's maximum in steps of 2^-11 powers of two (a probability is off
 //               by 2^-12.5 at most, an eighth of what P's own rounding to BF16 allows);
-//   loss_probs_kernel joins a row's pairs and turns its codes into P in place.
+//   loss_probs_kernel turns the codes into P in place once the rows' sums are known.
 //
 // Rows whose target is the ignored id take no part: the kept rows are first gathered into
 // consecutive ones (their number stays on the device), so padding costs no products and whatever
@@ -180,7 +180,7 @@ constexpr float kHalfLift = 32768.f;
 constexpr float kCodeSteps = 2048.f;  // of a code, to a power of two
 // Steps of K (1024 features) after which a tile of logits goes to registers and is added there.  The
 // tensor cores truncate as they add, which shrinks a logit by about D 10^-9 of itself: at 4096
-// features the loss was off by 1.8e-6, in segments of 1024 by MEASURE.
+// features the loss was off by 1.8e-6, in segments of 1024 by 4e-7.
 constexpr int kSegmentSteps = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -778,40 +778,7 @@ loss_slices_kernel(const float* __restrict__ slices, int count, const int32_t* k
 
 constexpr int kJoinThreads = 256;
 
-// log2 of a row's sum of exponentials from its (max, sum) pairs, by one CTA, in a fixed order: the
-// loss is the same bits whether its gradients are formed beside it or not.
-struct RowJoin {
-  float top, sum;
-  __device__ __forceinline__ void add(float other_top, float other_sum) {
-    const float high = fmaxf(top, other_top), pivot = high == -INFINITY ? 0.f : high;
-    sum = sum * exp2f(top - pivot) + other_sum * exp2f(other_top - pivot);
-    top = high;
-  }
-};
-
-__device__ __forceinline__ float join_row(const float2* mine, int pairs, float at_target) {
-  __shared__ RowJoin parts[kJoinThreads / 32];
-  const int tid = threadIdx.x;
-  RowJoin row{-INFINITY, 0.f};
-  for (int i = tid; i < pairs; i += kJoinThreads) {
-    const float2 v = __ldcg(mine + i);
-    row.add(v.x, v.y);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    row.add(__shfl_xor_sync(0xffffffffu, row.top, o), __shfl_xor_sync(0xffffffffu, row.sum, o));
-  __syncthreads();  // the previous row's use of `parts` is over
-  if ((tid & 31) == 0) parts[tid >> 5] = row;
-  __syncthreads();
-  row = parts[0];
-#pragma unroll
-  for (int w = 1; w < kJoinThreads / 32; ++w) row.add(parts[w].top, parts[w].sum);
-  // No logit at the target (an id outside the vocabulary): the loss and the gradients of the
-  // row are not numbers, so the mistake shows.
-  return isnan(at_target) ? at_target : row.top + log2f(row.sum);
-}
-
-// One CTA a kept row: its normaliser and its loss.
+// log2 of a row's sum of exponentials from its (max, sum) pairs, and its loss: one warp a kept row.
 __global__ void __launch_bounds__(kJoinThreads)
 loss_join_kernel(const float2* __restrict__ partials, int pairs, const int32_t* count, int first_row,
                  int row_limit, const float* __restrict__ target_logit,
@@ -819,57 +786,98 @@ loss_join_kernel(const float2* __restrict__ partials, int pairs, const int32_t* 
                  float* __restrict__ losses) {
   start_next_kernel();
   wait_for_previous_kernel();
-  const int rows = min(max(*count - first_row, 0), row_limit);
-  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
-    const float at_target = target_logit[first_row + row];
-    const float joined = join_row(partials + (int64_t)row * pairs, pairs, at_target);
-    if (threadIdx.x == 0) {
-      lse2[first_row + row] = joined;
-      losses[kept_index[first_row + row]] = (joined - at_target) * kLn2;
+  const int row = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= row_limit || first_row + row >= *count) return;
+  const float2* mine = partials + (int64_t)row * pairs;
+  float top = -INFINITY, sum = 0.f;
+  auto add = [&](float other_top, float other_sum) {
+    const float high = fmaxf(top, other_top), pivot = high == -INFINITY ? 0.f : high;
+    sum = sum * exp2f(top - pivot) + other_sum * exp2f(other_top - pivot);
+    top = high;
+  };
+  for (int i = lane; i < pairs; i += 256) {  // eight pairs at once: one trip to memory, one maximum
+    float2 v[8];
+    float high = -INFINITY, part = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      v[k] = i + 32 * k < pairs ? mine[i + 32 * k] : make_float2(-INFINITY, 0.f);
+      high = fmaxf(high, v[k].x);
     }
+    const float pivot = high == -INFINITY ? 0.f : high;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) part = fmaf(v[k].y, exp2f(v[k].x - pivot), part);
+    add(high, part);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float other_top = __shfl_xor_sync(0xffffffffu, top, o);
+    const float other_sum = __shfl_xor_sync(0xffffffffu, sum, o);
+    add(other_top, other_sum);
+  }
+  if (lane == 0) {
+    const float at_target = target_logit[first_row + row];
+    // No logit at the target (an id outside the vocabulary): the loss and the gradients of the
+    // row are not numbers, so the mistake shows.
+    const float joined = isnan(at_target) ? at_target : top + log2f(sum);
+    lse2[first_row + row] = joined;
+    losses[kept_index[first_row + row]] = (joined - at_target) * kLn2;
   }
 }
 
-// The same, and the row's codes become P = p - [v = target] in place.  Memory bounds it: 4 bytes a
-// logit, 4.7 TB/s at 16 384 x 32 000 (445 us; taking the rows last first, for what L2 still holds
-// of them, was slower).
-__global__ void __launch_bounds__(kJoinThreads)
+// Codes become P = p - [v = target] in place: a CTA takes 8192 columns of one kept row, a thread four
+// chunks of eight, all loaded before the first is converted.  Memory bounds it: 4 bytes a logit.
+constexpr int kProbsThreads = 256;
+constexpr int kProbsChunks = 4;
+constexpr int kProbsColumns = kProbsThreads * kProbsChunks * 8;
+
+__global__ void __launch_bounds__(kProbsThreads)
 loss_probs_kernel(const float2* __restrict__ partials, int pairs, const int32_t* count, int first_row,
                   int row_limit, const float* __restrict__ target_logit,
-                  const int32_t* __restrict__ kept_target, const int32_t* __restrict__ kept_index,
-                  float* __restrict__ losses, unsigned short* codes, int64_t stride, int V) {
+                  const int32_t* __restrict__ kept_target, const float* __restrict__ lse2,
+                  unsigned short* codes, int64_t stride, int V) {
   // (The products' CTAs would take the L1 cache for their shared memory while they wait: they start
   // when this kernel's CTAs are done.)
   wait_for_previous_kernel();
-  const int tid = threadIdx.x, rows = min(max(*count - first_row, 0), row_limit);
-  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
-    const float2* mine = partials + (int64_t)row * pairs;
-    const float at_target = target_logit[first_row + row];
-    const float lse2 = join_row(mine, pairs, at_target);
-    if (tid == 0) losses[kept_index[first_row + row]] = (lse2 - at_target) * kLn2;
-    const int target = kept_target[first_row + row];
-    const float residue = exp2f(at_target - lse2) - 1.f;
-    uint4* chunks = reinterpret_cast<uint4*>(codes + (int64_t)row * stride);
-#pragma unroll 4
-    for (int c = tid; c < (V + 7) / 8; c += kJoinThreads) {
-      const uint4 raw = __ldcs(chunks + c);
-      const float base = __ldcg(&mine[c >> 4].x) - lse2;  // sixteen chunks to a half tile
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-      uint32_t out[4];
+  const int parts = (V + kProbsColumns - 1) / kProbsColumns, total = (V + 7) / 8;
+  const int row = blockIdx.x / parts, part = blockIdx.x - row * parts;
+  if (row >= row_limit || first_row + row >= *count) return;
+  uint4* chunks = reinterpret_cast<uint4*>(codes + (int64_t)row * stride);
+  const float2* mine = partials + (int64_t)row * pairs;
+  const int first = part * (kProbsThreads * kProbsChunks) + threadIdx.x;
+  uint4 raw[kProbsChunks];
+  float base[kProbsChunks];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        // 2^23 + code as a float, then minus 2^23: exact
-        const float lo = __uint_as_float(__byte_perm(w[k], 0x4b000000u, 0x7610)) - 8388608.f;
-        const float hi = __uint_as_float(__byte_perm(w[k], 0x4b000000u, 0x7632)) - 8388608.f;
-        float p0 = exp2_approx(fmaf(lo, -1.f / kCodeSteps, base));
-        float p1 = exp2_approx(fmaf(hi, -1.f / kCodeSteps, base));
-        const int column = c * 8 + 2 * k;
-        if (column == target) p0 = residue;
-        if (column + 1 == target) p1 = residue;
-        out[k] = pack_bf16x2(p0, p1);
-      }
-      chunks[c] = make_uint4(out[0], out[1], out[2], out[3]);
+  for (int k = 0; k < kProbsChunks; ++k) {
+    const int c = first + k * kProbsThreads;
+    if (c < total) {
+      raw[k] = __ldcs(chunks + c);
+      base[k] = __ldg(&mine[c >> 4].x);  // sixteen chunks to a half tile
     }
+  }
+  const float sum2 = lse2[first_row + row];
+  const float residue = exp2f(target_logit[first_row + row] - sum2) - 1.f;
+  const int target = kept_target[first_row + row];
+#pragma unroll
+  for (int k = 0; k < kProbsChunks; ++k) {
+    const int c = first + k * kProbsThreads;
+    if (c >= total) continue;
+    const float up = base[k] - sum2;
+    const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+    float p[8];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      // 2^23 + code as a float, then minus 2^23: exact
+      const float lo = __uint_as_float(__byte_perm(w[q], 0x4b000000u, 0x7610)) - 8388608.f;
+      const float hi = __uint_as_float(__byte_perm(w[q], 0x4b000000u, 0x7632)) - 8388608.f;
+      p[2 * q] = exp2_approx(fmaf(lo, -1.f / kCodeSteps, up));
+      p[2 * q + 1] = exp2_approx(fmaf(hi, -1.f / kCodeSteps, up));
+    }
+    if (c == target >> 3) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e == (target & 7)) p[e] = residue;
+    }
+    chunks[c] = pack8(p);
   }
 }
 
