@@ -64,9 +64,9 @@ int launch_embedding_backward(const EmbedParams& p, int sms, cudaStream_t cs) {
   const int64_t tiles = (p.N + p.tile - 1) / p.tile;
   const auto [lanes, blocks] = columns_of(p.D, gradient_columns<VECTOR>());
   const int64_t units = tiles * blocks;
-  const int per_cta = kEmbedThreads / lanes;
+  const int per_cta = kSumThreads / lanes;
   embedding_sum_kernel<VECTOR, WIDE>
-      <<<(unsigned)((units + per_cta - 1) / per_cta), kEmbedThreads, 0, cs>>>(p, lanes, blocks, tiles);
+      <<<(unsigned)((units + per_cta - 1) / per_cta), kSumThreads, 0, cs>>>(p, lanes, blocks, tiles);
   if (int st = launched()) return st;
   if (tiles == 1) return ATTNRES_B200_OK;
   constexpr int warps = kEmbedThreads / 32;

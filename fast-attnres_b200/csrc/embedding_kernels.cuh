@@ -323,14 +323,18 @@ embedding_early_kernel(const EmbedParams p, int element_bytes, int fill_ctas) {
 
 constexpr int kJoinBatch = 8;  // pieces in flight per lane
 
+// Small CTAs: registers (102) allow five to an SM, 640 threads against 512 in CTAs of 256, and the
+// last ones end closer together.
+constexpr int kSumThreads = 128;
+
 template <bool VECTOR, bool WIDE>
-__global__ void __launch_bounds__(kEmbedThreads)
+__global__ void __launch_bounds__(kSumThreads)
 embedding_sum_kernel(const EmbedParams p, int lanes, int blocks, int64_t tiles) {
   start_next_kernel();  // the joining waits for the end
   constexpr int E = gradient_columns<VECTOR>();
   constexpr int kSumBatch = VECTOR ? 8 : 16;  // rows in flight per lane
   const int lane = threadIdx.x % lanes;
-  const int64_t unit = (int64_t)blockIdx.x * (kEmbedThreads / lanes) + threadIdx.x / lanes;
+  const int64_t unit = (int64_t)blockIdx.x * (kSumThreads / lanes) + threadIdx.x / lanes;
   const int64_t tile = unit / blocks;
   const int column = first_column<VECTOR, E>((int)(unit % blocks), lanes, lane);
   const int count = owned_columns<VECTOR, E>(column, lanes, p.D);
