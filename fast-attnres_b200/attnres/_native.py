@@ -9,7 +9,7 @@ import ctypes
 from ctypes import c_char_p, c_float, c_int32, c_int64, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 
-ABI_VERSION = 4
+ABI_VERSION = 3
 FLAG_FORCE_GENERIC = 1
 FLAG_PREFER_STREAM = 2
 FLAG_ACCUMULATE_DV = 4

@@ -370,6 +370,11 @@ struct TileOrder {
   }
 };
 
+// 16 384 rows, 32 000 ids, BF16: kStats 753 us at 1024 features (1.43 PFLOP/s), kCodes 828, kGradients
+// 1570 (1.37 PFLOP/s); at 4096 features (14 750 rows) kCodes 2.72 ms (1.42), kGradients 5.45 ms (1.42).
+// Power bounds them: clocks fall to 1.56 GHz within 200 us and to 1.35 in a long run, where cuBLAS
+// keeps 1.38 PFLOP/s on this GPU.
+//
 // Warp 0 loads, warp 1 multiplies (in a pair: the first CTA's, for both), warps 2..9 take finished
 // tiles out of tensor memory while the next one is formed in its other half.
 // Maps: kGradients: P, head, kept rows; the others: kept rows, head, P or codes (to store).

@@ -12,6 +12,10 @@
 // columns in registers for the whole launch.  With 16-byte accesses a thread copies its own chunks
 // of the rows ahead into a shared-memory ring (cp.async: no barrier, each thread reads back only
 // what it copied itself), otherwise the next row waits in registers.
+//
+// DRAM bounds it.  BF16, 16 384 rows, forward / backward with parameter gradients: 1024 features
+// 11.4 / 22 us (5.9 / 4.5 TB/s), 4096 features 44 / 75 us (6.1 / 5.4 TB/s), of 6.6 for a copy;
+// FP32, 8192 x 8192: 94 / 141 us (5.7 TB/s); element by element, FP32 4099 x 1537: 10.7 / 18 us.
 #pragma once
 
 #include "typed_access.cuh"

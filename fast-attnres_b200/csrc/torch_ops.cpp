@@ -1,9 +1,9 @@
 // torch operators of LayerNorm, embedding and vocabulary loss over the C ABI, with their autograd.
 //
 // These operators also run on a handful of rows, where the host's share of a call is most of its
-// time.  Bound in C++ a training call costs the host less than half of the same call through
-// ctypes and a Python autograd function (measured on a GPU host, layer_norm on eight rows, forward
-// and backward: see the comment on the entry points in attnres/norm.py).
+// time.  layer_norm on eight rows, on a GPU host: 8.5 us a call, 18.9 through ctypes; forward and
+// backward 77 us against 134 with a Python autograd function (60 of them are torch's engine, which
+// takes 57 us for a multiplication and its gradient on that host).
 //
 // Per operator: `<name>_forward` and `<name>_backward` do the work (their fake kernels are in
 // Python, so a compiled graph holds these two), `<name>` is the differentiable call.

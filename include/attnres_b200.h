@@ -40,7 +40,7 @@
 extern "C" {
 #endif
 
-#define ATTNRES_B200_ABI_VERSION 4
+#define ATTNRES_B200_ABI_VERSION 3
 /* Envelope of the reference operator (src/attnres/_sources.py:12-13). */
 #define ATTNRES_B200_MAX_SOURCES 129
 #define ATTNRES_B200_MAX_WIDTH 8192

@@ -316,7 +316,7 @@ def test_linear_cross_entropy_in_pieces(rows, vocabulary, width, ignored):
     assert all(torch.equal(a, b) for a, b in zip(first, second)), "not the same bits twice"
 
 
-@pytest.mark.parametrize("layout", ["three axes", "padded rows", "odd offset", "strided features",
+@pytest.mark.parametrize("layout", ["one row", "three axes", "padded rows", "odd offset", "strided features",
                                     "expanded rows", "padded head", "transposed head", "odd head",
                                     "strided targets", "expanded upstream"])
 def test_linear_cross_entropy_layouts(layout):
@@ -324,7 +324,9 @@ def test_linear_cross_entropy_layouts(layout):
     options = {}
     wide = torch.randn(120, 200, device="cuda").to(BF16)
     head = (torch.randn(260, 200, device="cuda") / 8).to(BF16)
-    if layout == "three axes":
+    if layout == "one row":
+        hidden, targets = hidden[7], targets[7]
+    elif layout == "three axes":
         hidden, targets = hidden.view(4, 30, 64), targets.view(4, 30)
     elif layout == "padded rows":
         hidden = wide[:, :64]
