@@ -823,9 +823,10 @@ loss_join_kernel(const float2* __restrict__ partials, int pairs, const int32_t* 
     const float at_target = target_logit[first_row + row];
     // No logit at the target (an id outside the vocabulary): the loss and the gradients of the
     // row are not numbers, so the mistake shows.
-    const float joined = isnan(at_target) ? at_target : top + log2f(sum);
-    lse2[first_row + row] = joined;
-    losses[kept_index[first_row + row]] = (joined - at_target) * kLn2;
+    const float over = log2f(sum);
+    lse2[first_row + row] = isnan(at_target) ? at_target : top + over;
+    // The two large numbers first: a small loss keeps its digits.
+    losses[kept_index[first_row + row]] = ((top - at_target) + over) * kLn2;
   }
 }
 

@@ -207,6 +207,26 @@ def test_linear_cross_entropy_large_logits():
     _check(hidden, weight, targets, scale=-300.0, reduction="sum")
 
 
+@pytest.mark.parametrize("train", [False, True])
+def test_linear_cross_entropy_small_losses_keep_their_digits(train):
+    """A confident row: z = (a, 0, ..), exact in BF16, loss = log(1 + 6 exp(-a)).  The target's logit
+    is the maximum, so what is rounded is a sum just over one (2^-23 at most) and its logarithm."""
+    from attnres.loss import linear_cross_entropy
+    for width in (16, 512):
+        hidden = torch.zeros(40, width, device="cuda", dtype=BF16)
+        hidden[:, 3] = torch.arange(40, device="cuda") / 2
+        weight = torch.zeros(7, width, device="cuda", dtype=BF16)
+        weight[5, 3] = 1
+        targets = torch.full((40,), 5, device="cuda")
+        weight.requires_grad_(train)
+        want = torch.log1p(6 * torch.exp(-hidden[:, 3].double()))
+        got = linear_cross_entropy(hidden, weight, targets, reduction="none").detach().double()
+        assert ((got - want).abs() <= 2 * E * (1 + want)).all(), (got - want).abs().max()
+        for row in (10, 20, 30):
+            total = linear_cross_entropy(hidden[row:], weight, targets[row:], reduction="sum").item()
+            assert abs(total - want[row:].sum().item()) <= (40 - row) * 2 * E * (1 + want[row].item())
+
+
 def test_linear_cross_entropy_infinities_and_nan_in_a_row_that_counts():
     from attnres.loss import linear_cross_entropy
     hidden, weight, targets = _case(10, 300, 64, BF16)
