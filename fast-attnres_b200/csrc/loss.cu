@@ -93,8 +93,8 @@ struct LossPlan {
   int64_t padded_weight;  // bytes of a padded copy of the weight
   int64_t stats_rows, partials;
   int64_t piece, pieces;  // ids of a piece
-  int64_t slices;         // of dH, in each piece
-  int64_t probs, slices_out, weights;
+  int64_t slices, weight_slices;
+  int64_t probs, slices_out, weight_out, weights;
 };
 
 int64_t tiles_of(int64_t rows, int64_t columns, bool pair) {
@@ -104,6 +104,13 @@ int64_t tiles_of(int64_t rows, int64_t columns, bool pair) {
 // Pairs of CTAs load a third less for the same products; single CTAs make twice as many, smaller
 // tiles, which is what counts when there are few.
 bool use_pairs(int64_t tiles_of_pairs) { return tiles_of_pairs >= 296; }
+
+// Slices that a gradient's sum is cut into: few rows (or few ids) make few tiles, each a long sum over
+// the vocabulary (or the rows).  One for every SM, but of sixteen steps at least.
+int64_t slices_of(int64_t tiles, int64_t sum_over) {
+  const int64_t wanted = 148 / tiles, most = (sum_over + kTileK - 1) / kTileK / 16;
+  return wanted < 1 || most < 1 ? 1 : wanted < most ? wanted : most;
+}
 
 LossPlan plan_loss(int64_t N, int32_t V, int32_t D) {
   LossPlan plan;
@@ -120,15 +127,11 @@ LossPlan plan_loss(int64_t N, int32_t V, int32_t D) {
   plan.pieces = (V + plan.piece - 1) / plan.piece;
   const int64_t columns = plan.piece < V ? plan.piece : padded_width(V);
   plan.probs = align256(N * columns * 2);
-  // dH has few tiles when there are few rows, each a long sum over the vocabulary: cut it so that
-  // there is one for every SM, but into sums of sixteen steps at least.
-  const int64_t tiles = tiles_of(N, D, false), steps = (plan.piece + kTileK - 1) / kTileK;
-  plan.slices = 148 / tiles;
-  if (plan.slices > steps / 16) plan.slices = steps / 16;
-  if (plan.slices < 1) plan.slices = 1;
-  plan.slices_out = plan.slices * plan.pieces > 1
-                        ? align256(plan.slices * N * D * (int64_t)sizeof(float))
-                        : 0;
+  const int64_t numbers = (int64_t)sizeof(float) * D;
+  plan.slices = slices_of(tiles_of(N, D, false), plan.piece);
+  plan.slices_out = plan.slices * plan.pieces > 1 ? align256(plan.slices * N * numbers) : 0;
+  plan.weight_slices = plan.pieces > 1 ? 1 : slices_of(tiles_of(V, D, false), N);
+  plan.weight_out = plan.weight_slices > 1 ? align256(plan.weight_slices * V * numbers) : 0;
   plan.weights = align256((N + 1) * (int64_t)sizeof(float));
   return plan;
 }
@@ -136,7 +139,8 @@ LossPlan plan_loss(int64_t N, int32_t V, int32_t D) {
 // The forward that forms the gradients as well works on pieces of the rows.
 struct GradientPlan {
   int64_t piece, pieces;  // rows
-  int64_t partials, codes, weight_out;
+  int64_t slices, weight_slices;
+  int64_t partials, codes, slices_out, weight_out;
 };
 
 GradientPlan plan_gradients(int64_t N, int32_t V, int32_t D) {
@@ -150,7 +154,12 @@ GradientPlan plan_gradients(int64_t N, int32_t V, int32_t D) {
   const int64_t tiles_n = (V + kTileN - 1) / kTileN;
   plan.partials = align256(plan.piece * 2 * tiles_n * (int64_t)sizeof(float2));
   plan.codes = align256(plan.piece * (int64_t)padded_width(V) * 2);
-  plan.weight_out = plan.pieces > 1 ? align256((int64_t)V * D * (int64_t)sizeof(float)) : 0;
+  const int64_t numbers = (int64_t)sizeof(float) * D;
+  plan.slices = slices_of(tiles_of(plan.piece, D, false), V);
+  plan.slices_out = plan.slices > 1 ? align256(plan.slices * N * numbers) : 0;
+  plan.weight_slices = slices_of(tiles_of(V, D, false), plan.piece);
+  plan.weight_out =
+      plan.weight_slices * plan.pieces > 1 ? align256(plan.weight_slices * V * numbers) : 0;
   return plan;
 }
 
@@ -195,6 +204,34 @@ int launch_product_type(int32_t type, const CUtensorMap (&maps)[3], const Produc
               : launch_product<PASS, __half, false>(maps, p, tiles(false), sms, stream);
 }
 
+// The gradients that were formed in parts.
+template <typename T>
+int launch_slices_type(const ProductParams& p, int sms, cudaStream_t stream) {
+  const int64_t most = 8 * sms, blocks = (p.D + kSliceColumns - 1) / kSliceColumns;
+  if (p.slices_out != nullptr) {
+    const int64_t ctas = (p.N * blocks + 7) / 8;
+    if (int st = launch_behind(loss_slices_kernel<T>, ctas < most ? ctas : most, 256, 0, true, stream,
+                               p.slices_out, p.slices, p.count, p.kept_index, p.gradient_scale,
+                               p.scale, (int64_t)p.N, p.D, static_cast<T*>(p.dhidden),
+                               p.vector_dhidden))
+      return st;
+  }
+  if (p.weight_out != nullptr) {
+    const int64_t ctas = (p.V * blocks + 7) / 8;
+    if (int st = launch_behind(loss_slices_kernel<T>, ctas < most ? ctas : most, 256, 0, true, stream,
+                               p.weight_out, p.weight_slices, nullptr, nullptr, p.gradient_scale,
+                               p.scale, (int64_t)p.V, p.D, static_cast<T*>(p.dweight),
+                               p.vector_dweight))
+      return st;
+  }
+  return ATTNRES_B200_OK;
+}
+
+int launch_slices(const ProductParams& p, int32_t type, int sms, cudaStream_t stream) {
+  return type == ATTNRES_B200_BF16 ? launch_slices_type<__nv_bfloat16>(p, sms, stream)
+                                   : launch_slices_type<__half>(p, sms, stream);
+}
+
 // The weight as the TMA can read it: in place, or copied into rows of a multiple of eight.
 int lay_out_weight(const void** weight, int64_t* row_stride, int32_t V, int32_t D, void* copy,
                    bool behind, int sms, cudaStream_t stream) {
@@ -223,10 +260,10 @@ extern "C" int64_t attnres_b200_loss_workspace_bytes(int64_t N, int32_t V, int32
   if (pass == ATTNRES_B200_LOSS_FORWARD_GRADIENTS) {
     const GradientPlan gradients = plan_gradients(N, V, D);
     return plan.padded_weight + gradients.partials + 2 * logits + 256 + gradients.codes +
-           gradients.weight_out;
+           gradients.slices_out + gradients.weight_out;
   }
   if (pass != ATTNRES_B200_LOSS_BACKWARD) return -ATTNRES_B200_ERR_BAD_FLAGS;
-  return plan.padded_weight + plan.probs + plan.slices_out + plan.weights;
+  return plan.padded_weight + plan.probs + plan.slices_out + plan.weight_out + plan.weights;
 }
 
 extern "C" int attnres_b200_loss_forward(
@@ -268,7 +305,8 @@ extern "C" int attnres_b200_loss_forward(
   float* sums = gradient_scale + 64;
   rest += 256 + align256(N * (int64_t)sizeof(float));
   unsigned short* codes = reinterpret_cast<unsigned short*>(rest);
-  float* weight_out = reinterpret_cast<float*>(rest + pieces.codes);
+  float* slices_out = reinterpret_cast<float*>(rest + pieces.codes);
+  float* weight_out = reinterpret_cast<float*>(rest + pieces.codes + pieces.slices_out);
 
   GatherParams g{};
   g.hidden = hidden;
@@ -325,7 +363,10 @@ extern "C" int attnres_b200_loss_forward(
     p.dweight = dweight;
     p.vector_dhidden = D % 8 == 0 && aligned16(dhidden);
     p.vector_dweight = D % 8 == 0 && aligned16(dweight);
-    p.slices = 1;
+    p.slices = (int32_t)pieces.slices;
+    p.weight_slices = (int32_t)pieces.weight_slices;
+    p.slices_out = dhidden != nullptr && pieces.slices_out > 0 ? slices_out : nullptr;
+    p.weight_out = dweight != nullptr && pieces.weight_out > 0 ? weight_out : nullptr;
     for (int64_t piece = 0; piece < pieces.pieces; ++piece) {
       p.first_row = (int32_t)(piece * pieces.piece);
       p.row_limit = (int32_t)(N - p.first_row < pieces.piece ? N - p.first_row : pieces.piece);
@@ -343,20 +384,14 @@ extern "C" int attnres_b200_loss_forward(
                                  partials, pairs, count, p.first_row, p.row_limit, target_logit,
                                  kept_target, sums, codes, stride, V))
         return st;
-      p.weight_out = dweight != nullptr && pieces.pieces > 1 ? weight_out : nullptr;
-      p.add = piece > 0;
+      p.add_weight = piece > 0;  // a piece's rows of dH are its own
       const auto both = [&](bool pair) {
-        return (dhidden ? tiles_of(p.row_limit, D, pair) : 0) + (dweight ? tiles_of(V, D, pair) : 0);
+        return (dhidden ? tiles_of(p.row_limit, D, pair) * p.slices : 0) +
+               (dweight ? tiles_of(V, D, pair) * p.weight_slices : 0);
       };
       if (int st = launch_product_type<kGradients>(type, use, p, both, sms, cs)) return st;
     }
-    if (p.weight_out != nullptr) {
-      if (int st = launch_behind(loss_slices_kernel<__nv_bfloat16>, 8 * sms, 256, 0, true, cs,
-                                 weight_out, 1, nullptr, nullptr, gradient_scale,
-                                 scale, (int64_t)V, D, static_cast<__nv_bfloat16*>(dweight),
-                                 p.vector_dweight))
-        return st;
-    }
+    if (int st = launch_slices(p, type, sms, cs)) return st;
   }
   for (int64_t row = 0; row < N && !gradients; row += plan.stats_rows) {
     p.first_row = (int32_t)row;
@@ -400,8 +435,10 @@ extern "C" int attnres_b200_loss_backward(
   char* space = static_cast<char*>(workspace);
   void* probs = space + plan.padded_weight;
   float* slices_out = reinterpret_cast<float*>(space + plan.padded_weight + plan.probs);
-  float* gradient_scale =
+  float* weight_out =
       reinterpret_cast<float*>(space + plan.padded_weight + plan.probs + plan.slices_out);
+  float* gradient_scale = reinterpret_cast<float*>(space + plan.padded_weight + plan.probs +
+                                                   plan.slices_out + plan.weight_out);
   float* weight_of = gradient_scale + 1;
 
   const bool padded = needs_padding(weight, weight_row_stride, V, D);
@@ -435,7 +472,9 @@ extern "C" int attnres_b200_loss_backward(
   p.vector_dhidden = D % 8 == 0 && aligned16(dhidden);
   p.vector_dweight = D % 8 == 0 && aligned16(dweight);
   p.slices = (int32_t)plan.slices;
-  p.slices_out = plan.slices_out > 0 ? slices_out : nullptr;
+  p.weight_slices = (int32_t)plan.weight_slices;
+  p.slices_out = dhidden != nullptr && plan.slices_out > 0 ? slices_out : nullptr;
+  p.weight_out = dweight != nullptr && plan.weight_out > 0 ? weight_out : nullptr;
   for (int64_t v0 = 0; v0 < V; v0 += plan.piece) {
     p.v0 = (int32_t)v0;
     p.vn = (int32_t)(V - v0 < plan.piece ? V - v0 : plan.piece);
@@ -447,21 +486,12 @@ extern "C" int attnres_b200_loss_backward(
     if (int st = launch_product_type<kProbs>(type, form, p, logits, sms, cs)) return st;
     const auto gradients = [&](bool pair) {
       return (dhidden ? tiles_of(N, D, pair) * plan.slices : 0) +
-             (dweight ? tiles_of(p.vn, D, pair) : 0);
+             (dweight ? tiles_of(p.vn, D, pair) * plan.weight_slices : 0);
     };
     if (int st = launch_product_type<kGradients>(type, use, p, gradients, sms, cs)) return st;
-    p.add = 1;
+    p.add_hidden = 1;  // a piece's rows of dW are its own
   }
-  if (dhidden == nullptr || p.slices_out == nullptr) return ATTNRES_B200_OK;
-  const int64_t ctas = (N + 7) / 8;
-  const unsigned grid = (unsigned)(ctas < 8 * sms ? ctas : 8 * sms);
-  if (type == ATTNRES_B200_BF16)
-    return launch_behind(loss_slices_kernel<__nv_bfloat16>, grid, 256, 0, true, cs, slices_out,
-                         p.slices, count, kept_index, gradient_scale, scale, N, D,
-                         static_cast<__nv_bfloat16*>(dhidden), p.vector_dhidden);
-  return launch_behind(loss_slices_kernel<__half>, grid, 256, 0, true, cs, slices_out, p.slices,
-                       count, kept_index, gradient_scale, scale, N, D, static_cast<__half*>(dhidden),
-                       p.vector_dhidden);
+  return launch_slices(p, type, sms, cs);
 }
 
 extern "C" int32_t attnres_b200_loss_gradients_in_forward(int32_t D, int32_t type, int32_t reduction) {

@@ -202,9 +202,9 @@ struct ProductParams {
   void* dhidden;           // kGradients: [N, D] or NULL
   void* dweight;           // kGradients: [V, D] or NULL
   float* slices_out;       // dH in several slices of the vocabulary: FP32 [slices][N, D], or NULL
-  int32_t slices;          // that a piece's sum for dH is cut into
-  float* weight_out;       // dW from several pieces of the rows: FP32 [V, D], or NULL
-  int32_t add;             // not the first piece: slices_out and weight_out are added to
+  float* weight_out;       // dW in several slices or pieces of the rows: FP32 [slices][V, D], or NULL
+  int32_t slices, weight_slices;  // that a piece's sums for dH and dW are cut into
+  int32_t add_hidden, add_weight;  // not the first piece: slices_out, or weight_out, is added to
   int32_t vector_dhidden, vector_dweight;  // their rows allow 16-byte stores
 };
 
@@ -303,7 +303,7 @@ struct Tile {
   int m, n;           // first row and column of the result
   int k_first, k_steps;
   bool weight;        // kGradients: dW rather than dH
-  int slice;          // of dH
+  int slice;          // of its sum
 };
 
 // The tiles of a launch in the order in which CTAs take them.  z: 2048 rows share each column tile
@@ -314,7 +314,7 @@ struct TileOrder {
   static constexpr int kRows = tile_rows(PAIR);
   int tiles_m, tiles_n, steps;     // kGradients: of dH
   int width = kTileN;              // kGradients: columns of a tile, D spread evenly over the tiles
-  int weight_m, weight_steps, slice_steps;
+  int weight_m, weight_steps, slice_steps, weight_slice_steps;
   int hidden_tiles, total;
 
   __device__ TileOrder(const ProductParams& p, int rows) {
@@ -326,8 +326,9 @@ struct TileOrder {
       slice_steps = (steps + p.slices - 1) / p.slices;
       weight_m = p.dweight != nullptr ? (p.vn + kRows - 1) / kRows : 0;
       weight_steps = (rows + kTileK - 1) / kTileK;
+      weight_slice_steps = (weight_steps + p.weight_slices - 1) / p.weight_slices;
       hidden_tiles = tiles_m * tiles_n * p.slices;
-      total = hidden_tiles + weight_m * tiles_n;
+      total = hidden_tiles + weight_m * tiles_n * p.weight_slices;
     } else {
       tiles_m = (rows + kRows - 1) / kRows;
       tiles_n = (p.vn + kTileN - 1) / kTileN;
@@ -343,17 +344,13 @@ struct TileOrder {
     t.k_first = 0;
     if constexpr (PASS == kGradients) {
       t.weight = index >= hidden_tiles;
-      int rest = index;
-      if (t.weight) {
-        rest -= hidden_tiles;
-        t.k_steps = weight_steps;
-      } else {
-        const int per_slice = tiles_m * tiles_n;
-        t.slice = index / per_slice;
-        rest = index - t.slice * per_slice;
-        t.k_first = t.slice * slice_steps;
-        t.k_steps = max(0, min(slice_steps, steps - t.k_first));
-      }
+      int rest = t.weight ? index - hidden_tiles : index;
+      const int per_slice = (t.weight ? weight_m : tiles_m) * tiles_n;
+      const int length = t.weight ? weight_slice_steps : slice_steps;
+      t.slice = rest / per_slice;
+      rest -= t.slice * per_slice;
+      t.k_first = t.slice * length;
+      t.k_steps = max(0, min(length, (t.weight ? weight_steps : steps) - t.k_first));
       const int row = rest / tiles_n;
       t.m = row * kRows;
       t.n = (rest - row * tiles_n) * width;
@@ -659,9 +656,9 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
         // A part of the sum, in FP32: loss_slices_kernel adds the slices and rounds.
         int64_t place = -1;
         if (t.weight) {
-          if (row < p.vn) place = (int64_t)(p.v0 + row) * p.D + column;
+          if (row < p.vn) place = ((int64_t)t.slice * p.V + p.v0 + row) * p.D + column;
         } else if (row < kept) {
-          place = ((int64_t)t.slice * p.N + row) * p.D + column;
+          place = ((int64_t)t.slice * p.N + p.first_row + row) * p.D + column;
         }
         float* parts = t.weight ? p.weight_out : p.slices_out;
 #pragma unroll 1
@@ -676,7 +673,8 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
             else
               store_shared16(block_slot(staging, lane, q), 0u, 0u, 0u, 0u);
           }
-          write_block<float>(staging, parts + c, place, columns - c, p.D % 4 == 0, lane, p.add);
+          write_block<float>(staging, parts + c, place, columns - c, p.D % 4 == 0, lane,
+                             t.weight ? p.add_weight : p.add_hidden);
         }
       } else {
         int64_t place = -1;
@@ -727,8 +725,12 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_0,
   if constexpr (PAIR) cluster_barrier();
 }
 
-// A gradient from its parts, added in order; one warp a row.  dH: the kept rows, to their places in
-// the input.  dW (no `kept_index`): rows as they are.
+// A gradient from its parts, added in order; a warp takes kSliceColumns of a row at a time, so that a
+// gradient of three rows still fills the GPU (10 rows of 1590 in 21 parts: 170 us with a warp a row,
+// 12 us so).  dH: the kept rows, to their places in the input.  dW (no `kept_index`): rows as
+// they are.
+constexpr int kSliceColumns = 256;
+
 template <typename T>
 __global__ void __launch_bounds__(256)
 loss_slices_kernel(const float* __restrict__ slices, int count, const int32_t* kept_rows,
@@ -740,41 +742,47 @@ loss_slices_kernel(const float* __restrict__ slices, int count, const int32_t* k
   const int lane = threadIdx.x & 31;
   const int64_t kept = kept_index != nullptr ? *kept_rows : N;
   const int64_t all = N * D;
-  for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < kept;
-       row += (int64_t)gridDim.x * 8) {
+  const int blocks = (D + kSliceColumns - 1) / kSliceColumns;
+  for (int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); item < kept * blocks;
+       item += (int64_t)gridDim.x * 8) {
+    const int64_t row = item / blocks;
+    const int first = (int)(item - row * blocks) * kSliceColumns;
     const float* mine = slices + row * D;
     T* to = out + (kept_index != nullptr ? kept_index[row] : row) * D;
+    float sum[8] = {};
     if (vector) {
-#pragma unroll 2
-      for (int c = lane * 8; c < D; c += 256) {
-        float sum[8] = {};
+      const int c = first + lane * 8;
+      if (c >= D) continue;
 #pragma unroll 4
-        for (int s = 0; s < count; ++s) {
-          const float4* from = reinterpret_cast<const float4*>(mine + s * all + c);
-          const float4 a = __ldcs(from), b = __ldcs(from + 1);
-          sum[0] += a.x;
-          sum[1] += a.y;
-          sum[2] += a.z;
-          sum[3] += a.w;
-          sum[4] += b.x;
-          sum[5] += b.y;
-          sum[6] += b.z;
-          sum[7] += b.w;
-        }
-        uint4 v;
-        v.x = pack2<T>(sum[0] * out_scale, sum[1] * out_scale);
-        v.y = pack2<T>(sum[2] * out_scale, sum[3] * out_scale);
-        v.z = pack2<T>(sum[4] * out_scale, sum[5] * out_scale);
-        v.w = pack2<T>(sum[6] * out_scale, sum[7] * out_scale);
-        *reinterpret_cast<uint4*>(to + c) = v;
+      for (int s = 0; s < count; ++s) {
+        const float4* from = reinterpret_cast<const float4*>(mine + s * all + c);
+        const float4 a = __ldcs(from), b = __ldcs(from + 1);
+        sum[0] += a.x;
+        sum[1] += a.y;
+        sum[2] += a.z;
+        sum[3] += a.w;
+        sum[4] += b.x;
+        sum[5] += b.y;
+        sum[6] += b.z;
+        sum[7] += b.w;
       }
+      uint4 v;
+      v.x = pack2<T>(sum[0] * out_scale, sum[1] * out_scale);
+      v.y = pack2<T>(sum[2] * out_scale, sum[3] * out_scale);
+      v.z = pack2<T>(sum[4] * out_scale, sum[5] * out_scale);
+      v.w = pack2<T>(sum[6] * out_scale, sum[7] * out_scale);
+      *reinterpret_cast<uint4*>(to + c) = v;
     } else {
-      for (int c = lane; c < D; c += 32) {
-        float sum = 0.f;
-#pragma unroll 4
-        for (int s = 0; s < count; ++s) sum += __ldcs(mine + s * all + c);
-        to[c] = from_float<T>(sum * out_scale);
+      const int c = first + lane;
+#pragma unroll 2
+      for (int s = 0; s < count; ++s) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + 32 * i < D) sum[i] += __ldcs(mine + s * all + c + 32 * i);
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + 32 * i < D) to[c + 32 * i] = from_float<T>(sum[i] * out_scale);
     }
   }
 }

@@ -336,6 +336,49 @@ def test_linear_cross_entropy_in_pieces(rows, vocabulary, width, ignored):
     assert all(torch.equal(a, b) for a, b in zip(first, second)), "not the same bits twice"
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("rows,vocabulary,width", [
+    (10, 30001, 520),       # dH in slices of the vocabulary, beside the logits and after them
+    (3, 9000, 1030),
+    (2600, 13, 40),         # dW in slices of the rows
+    (5001, 130, 515),
+    (2048, 2050, 77),       # one slice each of dH, two of dW
+    (2500, 2500, 512),      # both
+])
+def test_linear_cross_entropy_gradients_in_slices(rows, vocabulary, width, dtype):
+    hidden, weight, targets = _case(rows, vocabulary, width, dtype, ignored=0.1, seed=21)
+    first = _check(hidden, weight, targets, reduction="sum")
+    second = _check(hidden, weight, targets, reduction="sum")
+    assert all(torch.equal(a, b) for a, b in zip(first, second)), "not the same bits twice"
+    # a few kept rows leave most slices of dW empty, and none leaves them all so
+    from attnres.loss import linear_cross_entropy
+    targets[3:] = -100
+    _check(hidden.detach(), weight.detach(), targets)
+    loss = linear_cross_entropy(hidden, weight, torch.full_like(targets, -100), reduction="sum")
+    dhidden, dweight = torch.autograd.grad(loss, (hidden, weight))
+    assert loss == 0 and not dhidden.any() and not dweight.any()
+
+
+@pytest.mark.parametrize("rows,vocabulary,width", [
+    (1000, 600000, 512),    # two pieces of the rows, dH in slices in each
+    (180000, 3000, 512),    # two pieces of the rows, dW in slices in each
+])
+def test_linear_cross_entropy_slices_in_pieces(rows, vocabulary, width):
+    _check(*_case(rows, vocabulary, width, BF16, ignored=0.1, seed=22))
+
+
+@pytest.mark.parametrize("needed", ["hidden", "weight"])
+@pytest.mark.parametrize("rows,vocabulary,width", [(20, 9000, 520), (20, 9000, 72), (3000, 30, 520), (3000, 30, 72)])
+def test_linear_cross_entropy_slices_of_the_gradient_that_is_wanted(needed, rows, vocabulary, width):
+    from attnres.loss import linear_cross_entropy
+    hidden, weight, targets = _case(rows, vocabulary, width, BF16, seed=23)
+    both = _check(hidden, weight, targets)
+    hidden, weight = hidden.detach(), weight.detach()
+    leaf = (hidden if needed == "hidden" else weight).requires_grad_()
+    got, = torch.autograd.grad(linear_cross_entropy(hidden, weight, targets), leaf)
+    assert torch.equal(got, both[1 if needed == "hidden" else 2])
+
+
 @pytest.mark.parametrize("layout", ["one row", "three axes", "padded rows", "odd offset", "strided features",
                                     "expanded rows", "padded head", "transposed head", "odd head",
                                     "strided targets", "expanded upstream"])
@@ -459,7 +502,7 @@ def test_linear_cross_entropy_compiles_and_captures(width):
 def test_linear_cross_entropy_writes_only_its_outputs():
     from attnres import _native
     pad = 64
-    for rows, vocabulary, width in ((130, 300, 64), (67, 259, 37)):
+    for rows, vocabulary, width in ((130, 300, 64), (67, 259, 37), (3, 5003, 41), (4001, 5, 72)):
         hidden, weight, targets = _case(rows, vocabulary, width, BF16, ignored=0.3, seed=13)
         padded = (width + 7) // 8 * 8
 
