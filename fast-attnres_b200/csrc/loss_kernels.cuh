@@ -272,25 +272,35 @@ __device__ __forceinline__ void write_block(uint32_t staging, T* out, int64_t mi
       }
     }
   } else {
-    for (int row = 0; row < 32; ++row) {
-      const int64_t offset = __shfl_sync(0xffffffffu, mine, row);
-      if (offset < 0) continue;
+    // Element by element, eight rows' loads before their stores.
+    constexpr int each = width / 32;
+#pragma unroll 1
+    for (int first = 0; first < 32; first += 8) {
+      uint32_t v[8][each];
 #pragma unroll
-      for (int c = 0; c < width; c += 32) {
-        const int column = c + lane;
-        const uint32_t slot =
-            block_slot(staging, row, column / per_chunk) + column % per_chunk * (int)sizeof(T);
-        if (column < columns) {
-          if constexpr (sizeof(T) == 4) {
-            float v;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(slot) : "memory");
-            if (add) v = (float)out[offset + column] + v;
-            out[offset + column] = v;
-          } else {
-            unsigned short v;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(slot) : "memory");
-            reinterpret_cast<unsigned short*>(out)[offset + column] = v;
-          }
+      for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int e = 0; e < each; ++e) {
+          const int column = e * 32 + lane;
+          const uint32_t slot = block_slot(staging, first + i, column / per_chunk) +
+                                column % per_chunk * (int)sizeof(T);
+          if constexpr (sizeof(T) == 4)
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[i][e]) : "r"(slot));
+          else
+            asm volatile("ld.shared.u16 %0, [%1];" : "=r"(v[i][e]) : "r"(slot));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t offset = __shfl_sync(0xffffffffu, mine, first + i);
+#pragma unroll
+        for (int e = 0; e < each; ++e) {
+          const int column = e * 32 + lane;
+          if (offset < 0 || column >= columns) continue;
+          if constexpr (sizeof(T) == 4)
+            out[offset + column] = __uint_as_float(v[i][e]) + (add ? (float)out[offset + column] : 0.f);
+          else
+            reinterpret_cast<unsigned short*>(out)[offset + column] = (unsigned short)v[i][e];
         }
       }
     }
