@@ -58,18 +58,42 @@ __device__ __forceinline__ int64_t load_target(const void* targets, int wide, in
               : (int64_t)__ldg(static_cast<const int*>(targets) + n);
 }
 
+// Eight 16-bit elements from any even address, `count` of them in the row: words where the address
+// allows, so that nothing beyond the elements is read.  The rest are zeros.
+__device__ __forceinline__ uint4 load_eight(const unsigned short* src, int count) {
+  uint32_t w[4] = {};
+  if (count < 8) {
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (i < count) w[i / 2] |= (uint32_t)__ldg(src + i) << (i % 2 * 16);
+  } else if ((reinterpret_cast<uintptr_t>(src) & 2) == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
+  } else {
+    uint32_t inner[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) inner[i] = __ldg(reinterpret_cast<const uint32_t*>(src + 1) + i);
+    w[0] = __byte_perm(__ldg(src), inner[0], 0x5410);
+    w[1] = __byte_perm(inner[0], inner[1], 0x5432);
+    w[2] = __byte_perm(inner[1], inner[2], 0x5432);
+    w[3] = __byte_perm(inner[2], __ldg(src + 7), 0x5432);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // One 16-bit row of D elements into a 16-byte aligned one of Dp, by one warp; NULL: zeros.
 template <bool VECTOR>
 __device__ __forceinline__ void copy_row(unsigned short* dst, const unsigned short* src, int D,
                                          int Dp, int lane) {
-  if (VECTOR && src != nullptr) {
+  uint4* to = reinterpret_cast<uint4*>(dst);
+  if (src == nullptr) {
+    for (int c = lane; c < Dp / 8; c += 32) to[c] = make_uint4(0, 0, 0, 0);
+  } else if constexpr (VECTOR) {
 #pragma unroll 8
-    for (int c = lane; c < Dp / 8; c += 32)
-      reinterpret_cast<uint4*>(dst)[c] = __ldg(reinterpret_cast<const uint4*>(src) + c);
+    for (int c = lane; c < Dp / 8; c += 32) to[c] = __ldg(reinterpret_cast<const uint4*>(src) + c);
   } else {
-#pragma unroll 16
-    for (int i = lane; i < Dp; i += 32)
-      dst[i] = (src != nullptr && i < D) ? __ldg(src + i) : (unsigned short)0;
+#pragma unroll 4
+    for (int c = lane; c < Dp / 8; c += 32) to[c] = load_eight(src + c * 8, D - c * 8);
   }
 }
 
