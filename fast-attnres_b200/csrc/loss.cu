@@ -106,7 +106,9 @@ int64_t tiles_of(int64_t rows, int64_t columns, bool pair) {
 bool use_pairs(int64_t tiles_of_pairs) { return tiles_of_pairs >= 296; }
 
 // Slices that a gradient's sum is cut into: few rows (or few ids) make few tiles, each a long sum over
-// the vocabulary (or the rows).  One for every SM, but of sixteen steps at least.
+// the vocabulary (or the rows).  One for every SM, but of sixteen steps at least.  Whole and cut, with
+// the adding up: 10 rows of 49115 ids of 1590 features 363 and 162 us, 19318 rows of 13 ids of 111
+// features 107 and 22 us; the step over 1531 rows of 10007 ids of 523 features 123 and 118 us.
 int64_t slices_of(int64_t tiles, int64_t sum_over) {
   const int64_t wanted = 148 / tiles, most = (sum_over + kTileK - 1) / kTileK / 16;
   return wanted < 1 || most < 1 ? 1 : wanted < most ? wanted : most;
