@@ -44,10 +44,13 @@ template <bool VECTOR, bool WIDE>
 int launch_embedding_backward(const EmbedParams& p, int sms, cudaStream_t cs) {
   static SmemGrant grant;
   int64_t fill_ctas = 0, position_ctas = 0;
-  if (p.dtable != nullptr) {
+  const bool few = p.dtable != nullptr && p.N <= kFewTokens;
+  if (p.dtable != nullptr && !few) {
     if (int st = prepare_kernel(embedding_sort_kernel, kSortSmem, grant)) return st;
     embedding_sort_kernel<<<kSortCluster, kSortThreads, kSortSmem, cs>>>(p);
     if (int st = launched()) return st;
+  }
+  if (p.dtable != nullptr) {
     // Every filling CTA reads all ids: few of them where that takes longer than the filling.
     fill_ctas = p.N <= 65536 ? 4 * sms : sms;
     const int64_t ranges = ((int64_t)p.V + kFillRange - 2) / (kFillRange - 1);
@@ -56,9 +59,17 @@ int launch_embedding_backward(const EmbedParams& p, int sms, cudaStream_t cs) {
   }
   if (p.dpositions != nullptr)
     position_ctas = (p.T * ((p.D + 7) / 8) + kEarlyThreads - 1) / kEarlyThreads;
-  if (int st = launch_behind(embedding_early_kernel<VECTOR, WIDE>, fill_ctas + position_ctas,
+  if (few) {
+    const int64_t columns = 32 * gradient_columns<VECTOR>();
+    const int64_t sums = (p.N * ((p.D + columns - 1) / columns) * 32 + kEarlyThreads - 1) / kEarlyThreads;
+    embedding_early_kernel<VECTOR, WIDE, true>
+        <<<(unsigned)(fill_ctas + position_ctas + sums), kEarlyThreads, 0, cs>>>(
+            p, type_bytes(p.table_type), (int)fill_ctas, (int)sums);
+    return launched();
+  }
+  if (int st = launch_behind(embedding_early_kernel<VECTOR, WIDE, false>, fill_ctas + position_ctas,
                              kEarlyThreads, 0, p.dtable != nullptr, cs, p, type_bytes(p.table_type),
-                             (int)fill_ctas))
+                             (int)fill_ctas, 0))
     return st;
   if (p.dtable == nullptr) return ATTNRES_B200_OK;
   const int64_t tiles = (p.N + p.tile - 1) / p.tile;

@@ -113,6 +113,35 @@ def test_embed_gradient_is_summed_in_token_order():
     assert not grad[2].any() and not grad[[0, 1, 3]].any()
 
 
+@pytest.mark.parametrize("kind", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("width", [16, 37, 264, 1001, 2056])
+@pytest.mark.parametrize("n", [1, 31, 33, 127, 128, 129, 256])
+def test_embed_few_tokens(n, width, kind):
+    """Up to 128 tokens are not sorted."""
+    for vocabulary, ids in ((9, torch.full((n,), 8)), (5, torch.arange(n) * 7 % 5),
+                            (40000, 39999 - torch.arange(n)), (300, torch.arange(n) * n % 300)):
+        for padding_idx in (None, int(ids[n // 2])):
+            _, first = _check(ids.cuda()[None], _table(vocabulary, width, kind), _table(n, width, FP32, 3),
+                              scale=0.6, padding_idx=padding_idx, seed=n)
+            _, second = _check(ids.cuda()[None], _table(vocabulary, width, kind),
+                               _table(n, width, FP32, 3), scale=0.6, padding_idx=padding_idx, seed=n)
+            assert all(torch.equal(a, b) for a, b in zip(first, second)), "not the same bits twice"
+
+
+def test_embed_few_tokens_in_the_order_of_more():
+    """The sums are those of a sorted call where no run crosses a tile of 32."""
+    from attnres.embedding import embed
+    ids = torch.arange(120, device="cuda") * 17 % 47
+    upstream = _table(120, 72, FP32, 9)
+    grads = []
+    for extra in (0, 100):   # the others have no gradient
+        table = _table(47, 72, FP32).requires_grad_()
+        tokens = torch.cat((ids, torch.full((extra,), 1 << 20, device="cuda")))
+        more = torch.cat((upstream, upstream[:extra]))
+        grads.append(torch.autograd.grad(embed(tokens[None], table), table, more[None])[0])
+    assert torch.allclose(grads[0], grads[1], rtol=4 * U, atol=4 * U * 3 * upstream.abs().max().item())
+
+
 @pytest.mark.parametrize("n", [32, 33, 4096, 131073, 200000])
 def test_embed_many_tokens(n):
     """Past 131 072 tokens the tiles grow; the sort's shares are longer than a warp."""
@@ -248,8 +277,9 @@ def test_embed_compiles_and_captures():
 
 def test_embed_writes_only_its_outputs():
     from attnres import _native
-    n, period, vocabulary, pad = 300, 100, 77, 64
-    for width, code, dtype in ((64, 2, FP32), (37, 0, BF16), (1030, 1, FP16)):
+    period, vocabulary, pad = 100, 77, 64
+    for n, width, code, dtype in ((300, 64, 2, FP32), (300, 37, 0, BF16), (300, 1030, 1, FP16),
+                                  (100, 64, 0, BF16), (100, 1030, 2, FP32)):
         tokens, table = _ids((n,), vocabulary), _table(vocabulary, width, dtype)
 
         def guarded(count, kind):
