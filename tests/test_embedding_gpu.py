@@ -223,6 +223,81 @@ def test_embed_layouts(layout):
     _check(tokens, table, positions, upstream=upstream)
 
 
+@pytest.mark.parametrize("n", [100, 400])
+@pytest.mark.parametrize("layout", ["odd table", "transposed table", "strided ids", "sliced gradient",
+                                    "odd gradient", "expanded gradient"])
+def test_embed_layouts_sorted_and_not(layout, n):
+    tokens, table, positions, upstream = _ids((2, n // 2), 60), _table(60, 64, FP32), None, None
+    if layout == "odd table":
+        table = _table(60, 81, BF16)[:, 3:67]
+    elif layout == "transposed table":
+        table, positions = _table(64, 60, FP32).t(), _table(64, n // 2, FP32).t()
+    elif layout == "strided ids":
+        tokens = _ids((n // 2, 8), 60)[:, ::4].t()
+    elif layout == "sliced gradient":
+        upstream = torch.randn(2, n // 2, 72, device="cuda")[..., 4:68]
+    elif layout == "odd gradient":
+        upstream = torch.randn(2, n // 2, 67, device="cuda")[..., 3:]
+    else:
+        upstream = torch.ones((), device="cuda").expand(2, n // 2, 64)
+    _check(tokens, table, positions, upstream=upstream)
+
+
+@pytest.mark.parametrize("n", [90, 500])
+def test_embed_bad_ids_padding_and_infinities_sorted_and_not(n):
+    from attnres.embedding import embed
+    torch.manual_seed(3)
+    table = _table(50, 40, FP32).requires_grad_()
+    _, grads = _check(torch.full((2, n // 2), 3, device="cuda"), table.detach(), padding_idx=3)
+    assert not grads[0].any()
+    tokens, upstream = _ids((n,), 50), torch.randn(n, 40, device="cuda")
+    strange = torch.tensor([-1, 50, 2**40, -2**63, 2**31, 2**32 + 1, -2**31], device="cuda")
+    where = torch.randperm(n, device="cuda")[:7]
+    tokens[where] = strange
+    upstream[where] = float("nan")      # of rows without an id: reaches nothing
+    upstream[where[0] - 1] = float("inf")
+    hit = tokens[where[0] - 1]
+    grad, = torch.autograd.grad(embed(tokens, table), table, upstream)
+    fine = (tokens >= 0) & (tokens < 50) & (tokens != hit)
+    want = torch.zeros(50, 40, device="cuda", dtype=torch.float64)
+    want.index_add_(0, tokens[fine], upstream[fine].double())
+    size = torch.zeros_like(want).index_add_(0, tokens[fine], upstream[fine].abs().double())
+    if 0 <= int(hit) < 50:
+        assert grad[hit].isinf().all()
+        grad[hit] = 0
+    _inside(grad, want, (n + 4) * U * size, "dtable")
+
+
+@pytest.mark.parametrize("needed", ["table", "positions"])
+def test_embed_only_the_gradient_that_is_wanted_sorted(needed):
+    from attnres.embedding import embed
+    tokens, table, positions = _ids((3, 140), 70), _table(70, 24, FP32), _table(140, 24, FP32, 3)
+    leaf = (table if needed == "table" else positions).requires_grad_()
+    out = embed(tokens, table, positions)
+    got, = torch.autograd.grad(out, leaf, torch.ones_like(out))
+    want = torch.bincount(tokens.reshape(-1), minlength=70)[:, None].expand(70, 24) \
+        if needed == "table" else torch.full((140, 24), 3.0, device="cuda")
+    assert torch.equal(got, want.float())
+
+
+def test_embed_few_tokens_captured():
+    from attnres.embedding import embed
+    table = _table(500, 264, BF16).requires_grad_()
+    ids, upstream = _ids((1, 40), 500), _table(40, 264, BF16, 5)[None]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(embed(ids, table), table, upstream)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grad, = torch.autograd.grad(embed(ids, table), table, upstream)
+    ids.copy_(_ids((1, 40), 500, 9))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(grad, torch.autograd.grad(embed(ids, table), table, upstream)[0])
+
+
 def test_embed_no_tokens():
     from attnres.embedding import embed
     table, positions = _table(10, 16, BF16).requires_grad_(), _table(5, 16, BF16).requires_grad_()
