@@ -340,10 +340,12 @@ def test_linear_cross_entropy_in_pieces(rows, vocabulary, width, ignored):
 @pytest.mark.parametrize("rows,vocabulary,width", [
     (10, 30001, 520),       # dH in slices of the vocabulary, beside the logits and after them
     (3, 9000, 1030),
-    (2600, 13, 40),         # dW in slices of the rows
+    (1900, 13, 40),         # too short to be cut
+    (5201, 13, 40),         # dW in slices of the rows
     (5001, 130, 515),
-    (2048, 2050, 77),       # one slice each of dH, two of dW
-    (2500, 2500, 512),      # both
+    (2048, 9050, 77),       # more of dH than of dW
+    (6500, 6400, 512),      # tiles for every SM: none
+    (4600, 4500, 130),      # both
 ])
 def test_linear_cross_entropy_gradients_in_slices(rows, vocabulary, width, dtype):
     hidden, weight, targets = _case(rows, vocabulary, width, dtype, ignored=0.1, seed=21)
@@ -368,7 +370,7 @@ def test_linear_cross_entropy_slices_in_pieces(rows, vocabulary, width):
 
 
 @pytest.mark.parametrize("needed", ["hidden", "weight"])
-@pytest.mark.parametrize("rows,vocabulary,width", [(20, 9000, 520), (20, 9000, 72), (3000, 30, 520), (3000, 30, 72)])
+@pytest.mark.parametrize("rows,vocabulary,width", [(20, 9000, 520), (20, 9000, 72), (6000, 30, 520), (6000, 30, 72)])
 def test_linear_cross_entropy_slices_of_the_gradient_that_is_wanted(needed, rows, vocabulary, width):
     from attnres.loss import linear_cross_entropy
     hidden, weight, targets = _case(rows, vocabulary, width, BF16, seed=23)
@@ -502,7 +504,7 @@ def test_linear_cross_entropy_compiles_and_captures(width):
 def test_linear_cross_entropy_writes_only_its_outputs():
     from attnres import _native
     pad = 64
-    for rows, vocabulary, width in ((130, 300, 64), (67, 259, 37), (3, 5003, 41), (4001, 5, 72)):
+    for rows, vocabulary, width in ((130, 300, 64), (67, 259, 37), (3, 5003, 41), (6001, 5, 72)):
         hidden, weight, targets = _case(rows, vocabulary, width, BF16, ignored=0.3, seed=13)
         padded = (width + 7) // 8 * 8
 
